@@ -59,6 +59,8 @@ enum ErrorCode : int {
   kErrPeerTimeout = 5,
   kErrBadShape = 6,
   kErrBadIndex = 7,   // kernel-checks builds: an index outside its table (the access is clamped)
+  // In the second word (err[1]): what the inputs hold, which stops no kernel.
+  kErrBadToken = 8,   // a token id or target outside the vocabulary (nothing is read there)
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {

@@ -3,8 +3,10 @@
 The library is built in-tree (``python setup.py build_ext --inplace``).  On a
 machine with a GPU the fused path requires it: a missing or stale library is an
 error, never a silent fallback to PyTorch.  Each device gets a small int32
-error word that kernels set when a bounded wait gives up; ``check_errors``
-turns it into an exception at the next host synchronisation point.
+error word that kernels set when a bounded wait gives up (word 0) or when they
+meet a token id outside the vocabulary (word 1, which stops no kernel);
+``check_errors`` turns it into an exception at the next host synchronisation
+point.
 """
 
 from __future__ import annotations
@@ -22,11 +24,16 @@ ERROR_NAMES = {
     5: "peer GPU never signalled (cross-GPU flag timeout)",
     6: "bad shape",
     7: "index outside its table (kernel-checks build; the access was clamped)",
+    8: "token id or target outside the vocabulary (its row was left out)",
 }
 
 
 class KernelTimeout(RuntimeError):
     """A kernel's bounded wait expired; the kernel exited without finishing."""
+
+
+class KernelDataError(RuntimeError):
+    """A kernel met input values that it cannot use (it left them out)."""
 
 
 class LaunchCounter:
@@ -108,9 +115,13 @@ def err_word(device: torch.device | int | None = None) -> torch.Tensor:
 
 
 def check_errors(device: torch.device | int | None = None) -> None:
-    """Raise ``KernelTimeout`` if any kernel on ``device`` reported a failure."""
+    """Raise ``KernelTimeout`` if any kernel on ``device`` reported a failure,
+    ``KernelDataError`` if one met a token id outside the vocabulary."""
     word = err_word(device)
-    code = int(word[0].item())
+    code, data = word[:2].tolist()
     if code:
         word.zero_()
         raise KernelTimeout(f"kernel error {code}: {ERROR_NAMES.get(code, 'unknown')}")
+    if data:
+        word.zero_()
+        raise KernelDataError(f"kernel error {data}: {ERROR_NAMES.get(data, 'unknown')}")

@@ -397,3 +397,59 @@ def sample_append_split(logits, temperature, seed, next_ids, slot, pos, kv_len, 
         raise NotImplementedError("the vocab-parallel sampler exchange writes peer memory and needs GPUs")
     sample_append(logits, temperature, 1.0, seed, next_ids, slot, pos, kv_len, finished, out_tokens, prompt_slots,
                   eos_id, pad_id, ignore_eos, None)
+
+
+def ce_forward(h, W, targets, ignore_index, reduction, grad, with_scale, err):
+    T, H = h.shape
+    V = W.shape[0]
+    cap, Hp = max(-(-T // 128) * 128, 128), -(-H // 8) * 8
+    live = (targets != ignore_index) & (targets >= 0) & (targets < V)
+    bad = ~live & (targets != ignore_index)
+    if bool(bad.any()):
+        err[1] = 8
+    rows = live.nonzero()[:, 0]
+    n = rows.numel()
+    token = torch.full((cap,), -1, dtype=torch.int32)
+    token[:n] = rows.int()
+    place = torch.full((T,), -1, dtype=torch.int32)
+    place[rows] = torch.arange(n, dtype=torch.int32)
+    target = torch.zeros(cap, dtype=torch.int64)
+    target[:n] = targets[rows]
+    count = torch.tensor([n], dtype=torch.int32)
+    hc = torch.zeros(cap, Hp, dtype=h.dtype)
+    hc[:n, :H] = h[rows]
+    logits = _f(hc[:n, :H]) @ _f(W).T
+    lse = torch.zeros(cap)
+    lse[:n] = torch.logsumexp(logits, -1)
+    loss = torch.zeros(T)
+    loss[bad] = float("nan")
+    loss[rows] = lse[:n] - logits.gather(1, target[:n, None])[:, 0]
+    scale = torch.zeros(cap)
+    if grad is not None or with_scale:
+        ce_scale(token, count, torch.ones(1) if grad is None else grad, reduction, scale)
+    if reduction:
+        loss = loss.sum() / (max(1, n) if reduction == 2 else 1)
+    return loss, hc, token, place, target, count, lse, scale
+
+
+def ce_scale(token, count, grad, reduction, scale):
+    n = int(count)
+    up = grad[token[:n].long()] if grad.numel() != 1 else grad.expand(n)
+    scale[:n] = up / (n if reduction == 2 else 1)
+
+
+def ce_backward(hc, W, place, target, count, lse, scale, dh, dW, piece, err):
+    n, (V, H) = int(count), W.shape
+    piece = piece or V
+    h, acc = _f(hc[:n, :H]), torch.zeros(n, H)
+    for v0 in range(0, V, piece):
+        Wv = _f(W[v0 : v0 + piece])
+        cols = torch.arange(v0, v0 + Wv.shape[0])
+        hot = (target[:n, None] == cols).float()
+        d = (scale[:n, None] * (torch.exp(h @ Wv.T - lse[:n, None]) - hot)).to(hc.dtype).float()
+        acc += d @ Wv
+        if dW is not None:
+            dW[v0 : v0 + piece] = (d.T @ h).to(dW.dtype)
+    if dh is not None:
+        dh.zero_()
+        dh[place >= 0] = acc.to(dh.dtype)

@@ -1,0 +1,317 @@
+"""Cross entropy over a vocabulary projection (graspo_b200/ops/cross_entropy.py):
+losses and both gradients against the definition in 64 bits, element by element.
+
+Tolerances.  With bf16 operands every product is exact in fp32.  The tensor cores
+add 16 products per step, so a logit is off by at most
+``delta = (H / 16 + 16) * 2^-22 * max sum_k |h_k W_k|`` (one rounding or
+truncation of a partial sum per step).  The loss is the difference of two such
+values plus a log-sum-exp of fp32 exponentials (relative error below 2^-18).
+An entry of the softmax gradient d carries the logit's and the log-sum-exp's
+error (relative 3 delta + 2^-17) and one rounding to bf16 (8 significant bits:
+2^-8); dh and dW sum entries with those errors and are rounded to bf16 once more.
+"""
+
+import math
+
+import pytest
+import torch
+
+IGNORE = -100
+
+
+def _case(T, H, V, valid, seed=0, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(T, H, generator=g).to(torch.bfloat16)
+    w = (torch.randn(V, H, generator=g) * (2.0 / math.sqrt(H))).to(torch.bfloat16)
+    t = torch.randint(0, V, (T,), generator=g)
+    t[torch.rand(T, generator=g) >= valid] = IGNORE
+    up = torch.randn(T, generator=g)
+    return h.to(device), w.to(device), t.to(device), up.to(device)
+
+
+def _oracle(h, w, t, scale, ignore=IGNORE):
+    """(loss per token, dh, dw) and the elementwise error bounds, in 64 bits."""
+    live = t != ignore
+    hd, wd = torch.where(live[:, None], h.double(), 0.0), w.double()
+    logits = hd @ wd.T
+    lse = torch.logsumexp(logits, -1)
+    at = torch.where(live, t, 0)[:, None]
+    loss = torch.where(live, lse - logits.gather(1, at)[:, 0], 0.0)
+    p = torch.exp(logits - lse[:, None])
+    hot = torch.zeros_like(p).scatter_(1, at, 1.0)
+    s = torch.where(live, scale.double(), 0.0)[:, None]
+    d, size = (p - hot) * s, (p + hot) * s.abs()
+    H = h.shape[1]
+    delta = (H / 16 + 16) * 2.0 ** -22 * float((hd.abs() @ wd.abs().T).max())
+    rel = (2.0 ** -8 + 3 * delta + 2.0 ** -17) * (1 + 2.0 ** -8)
+    dh, dw = d @ wd, d.T @ hd
+    return loss, dh, dw, {
+        "loss": 2 * delta + 2.0 ** -18 * (1 + loss.abs()),
+        "dh": rel * (size @ wd.abs()) + 2.0 ** -8 * dh.abs() + 1e-30,
+        "dw": rel * (size.T @ hd.abs()) + 2.0 ** -8 * dw.abs() + 1e-30,
+    }
+
+
+def _within(got, want, bound, what):
+    assert got.shape == want.shape
+    off = (got.double() - want).abs() - bound
+    assert bool((off <= 0).all()), f"{what}: {int((off > 0).sum())} values outside, worst by {float(off.max()):.3g}"
+
+
+SHAPES = [
+    # tokens, hidden, vocabulary, share of trained tokens, piece
+    (1, 64, 256, 1.0, 0),
+    (1, 8, 1, 1.0, 0),              # one column: loss 0, gradient 0
+    (2, 1, 3, 1.0, 0),              # one hidden value
+    (61, 512, 4096, 0.8, 0),
+    (127, 72, 300, 1.0, 256),
+    (128, 64, 256, 1.0, 0),
+    (129, 200, 1000, 0.5, 256),
+    (333, 1001, 777, 0.6, 256),     # odd rows
+    (300, 136, 2055, 0.1, 512),
+    (1030, 264, 513, 0.97, 0),
+    (64, 512, 30001, 1.0, 0),       # the contraction over the vocabulary is split
+    (64, 512, 30001, 1.0, 8192),
+    (40, 64, 64, 0.0, 0),           # no trained token
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,V,valid,piece", SHAPES)
+def test_grads_against_64_bits(T, H, V, valid, piece):
+    from graspo_b200.ops._ext import check_errors
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(T, H, V, valid, seed=T)
+    loss, dh, dw = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none", piece=piece)
+    check_errors()
+    want, wh, ww, bound = _oracle(h, w, t, up)
+    assert loss.dtype == torch.float32 and dh.dtype == dw.dtype == torch.bfloat16
+    _within(loss, want, bound["loss"], "loss")
+    _within(dh, wh, bound["dh"], "dh")
+    _within(dw, ww, bound["dw"], "dw")
+    assert torch.equal(loss[t == IGNORE], torch.zeros_like(loss[t == IGNORE]))
+    assert not dh[t == IGNORE].any()
+    again = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none", piece=piece)
+    assert all(torch.equal(a, b) for a, b in zip((loss, dh, dw), again)), "two calls differ"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_autograd_reductions_and_batch_shape(reduction):
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy
+
+    h, w, t, up = _case(6 * 35, 128, 515, 0.7, seed=3)
+    hl, wl = h.view(6, 35, 128).clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(hl, wl, t.view(6, 35), reduction=reduction)
+    n = int((t != IGNORE).sum())
+    if reduction == "none":
+        assert loss.shape == (6, 35)
+        (loss * up.view(6, 35)).sum().backward()
+        scale = up
+    else:
+        (loss * 1.75).backward()
+        scale = torch.full_like(up, 1.75 / (n if reduction == "mean" else 1))
+    want, wh, ww, bound = _oracle(h, w, t, scale)
+    if reduction == "none":
+        _within(loss.detach().view(-1), want, bound["loss"], "loss")
+    else:
+        k = 1 / n if reduction == "mean" else 1
+        assert abs(float(loss.detach()) - float(want.sum()) * k) <= (float(bound["loss"].sum()) * k
+                                                                    + 2.0 ** -23 * float(want.sum()) * k)
+    _within(hl.grad.view(-1, 128), wh, bound["dh"], "dh")
+    _within(wl.grad, ww, bound["dw"], "dw")
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    """<dh, u> and <dW, u> against central differences of the 64-bit loss along u."""
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(50, 96, 700, 0.8, seed=9)
+    _, dh, dw = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none")
+    _, _, _, bound = _oracle(h, w, t, up)
+    g = torch.Generator().manual_seed(1)
+    u, q = torch.randn(h.shape, generator=g).cuda().double(), torch.randn(w.shape, generator=g).cuda().double()
+
+    def total(a, b):
+        live = t != IGNORE
+        logp = torch.log_softmax(a[live] @ b.T, -1)
+        return float((-logp.gather(1, t[live][:, None])[:, 0] * up[live].double()).sum())
+
+    e = 1e-5  # the next term of the difference is of the order e^2 times a third derivative of some 10^4
+    hd, wd = h.double(), w.double()
+    along_h = (total(hd + e * u, wd) - total(hd - e * u, wd)) / (2 * e)
+    along_w = (total(hd, wd + e * q) - total(hd, wd - e * q)) / (2 * e)
+    assert abs(float((dh.double() * u).sum()) - along_h) <= float((bound["dh"] * u.abs()).sum()) + 1e-4
+    assert abs(float((dw.double() * q).sum()) - along_w) <= float((bound["dw"] * q.abs()).sum()) + 1e-4
+
+
+@pytest.mark.gpu
+def test_ignored_rows_may_hold_anything():
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(200, 128, 600, 0.5, seed=4)
+    clean = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none")
+    dead = t == IGNORE
+    h2, up2 = h.clone(), up.clone()
+    h2[dead] = float("nan")
+    h2[dead.nonzero()[0]] = float("inf")
+    up2[dead] = float("nan")
+    dirty = linear_cross_entropy_grads(h2, w, t, grad=up2, reduction="none")
+    assert all(torch.equal(a, b) for a, b in zip(clean, dirty))
+
+
+@pytest.mark.gpu
+def test_other_ignore_index_and_int32_targets():
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(90, 64, 300, 1.0, seed=5)
+    t[::3] = 7
+    loss, dh, dw = linear_cross_entropy_grads(h, w, t.int(), grad=up, reduction="none", ignore_index=7)
+    want, wh, ww, bound = _oracle(h, w, t, up, ignore=7)
+    _within(loss, want, bound["loss"], "loss")
+    _within(dh, wh, bound["dh"], "dh")
+    _within(dw, ww, bound["dw"], "dw")
+
+
+@pytest.mark.gpu
+def test_target_outside_the_vocabulary():
+    from graspo_b200.ops._ext import KernelDataError, check_errors
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(70, 64, 300, 1.0, seed=6)
+    bad = t.clone()
+    bad[3], bad[40] = 300, -1
+    loss, dh, dw = linear_cross_entropy_grads(h, w, bad, grad=up, reduction="none")
+    with pytest.raises(KernelDataError):
+        check_errors()
+    check_errors()                                  # reported once
+    assert loss.isnan().nonzero()[:, 0].tolist() == [3, 40]
+    t[3] = t[40] = IGNORE
+    want, wh, ww, bound = _oracle(h, w, t, up)
+    ok = t != IGNORE
+    _within(loss[ok], want[ok], bound["loss"][ok], "loss")
+    _within(dh, wh, bound["dh"], "dh")
+    _within(dw, ww, bound["dw"], "dw")
+
+
+@pytest.mark.gpu
+def test_strides_offsets_and_another_stream():
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(100, 96, 520, 0.8, seed=7)
+    want = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none")
+    wide = torch.randn(100, 200, device="cuda").to(torch.bfloat16)
+    wide[:, 3:99] = h                               # rows that start off a 16-byte boundary
+    pad = torch.randn(520, 104, device="cuda").to(torch.bfloat16)
+    pad[:, :96] = w                                 # rows with a gap
+    off = torch.empty(520 * 96 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(520, 96)
+    off.copy_(w)
+    for hh in (wide[:, 3:99], h.T.contiguous().T):
+        for ww in (pad[:, :96], off, w.T.contiguous().T):
+            got = linear_cross_entropy_grads(hh, ww, t, grad=up, reduction="none")
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none")
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_large_logits_do_not_overflow():
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(64, 64, 512, 1.0, seed=8)
+    h = (h.float() * 60).to(torch.bfloat16)         # logits of some hundreds
+    loss, dh, dw = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none")
+    want, wh, ww, bound = _oracle(h, w, t, up)
+    _within(loss, want, bound["loss"], "loss")
+    _within(dh, wh, bound["dh"], "dh")
+    _within(dw, ww, bound["dw"], "dw")
+
+
+@pytest.mark.gpu
+def test_frozen_projection_and_no_trained_token():
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy, linear_cross_entropy_grads
+
+    h, w, t, _ = _case(30, 64, 256, 1.0)
+    loss, dh, dw = linear_cross_entropy_grads(h, w, t, weight_grad=False)
+    full = linear_cross_entropy_grads(h, w, t)
+    assert dw is None and torch.equal(loss, full[0]) and torch.equal(dh, full[1])
+    hl = h.clone().requires_grad_(True)
+    out = linear_cross_entropy(hl, w, torch.full_like(t, IGNORE))
+    out.backward()
+    assert float(out.detach()) == 0.0 and not hl.grad.any()
+    empty = linear_cross_entropy_grads(h[:0], w, t[:0])
+    assert float(empty[0]) == 0.0 and empty[1].shape == (0, 64) and not empty[2].any()
+
+
+def test_cpu_form_matches_64_bits():
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy, linear_cross_entropy_grads
+
+    h, w, t, up = _case(37, 24, 50, 0.6, device="cpu")
+    h, w = h.float(), w.float()
+    loss, dh, dw = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none")
+    want, wh, ww, _ = _oracle(h, w, t, up)
+    for a, b in ((loss, want), (dh, wh), (dw, ww)):      # fp32 sums of at most 50 terms of order 10
+        assert (a.double() - b).abs().max() < 50 * 2.0 ** -23 * 10
+    hl = h.clone().requires_grad_(True)
+    linear_cross_entropy(hl, w, torch.full_like(t, IGNORE)).backward()
+    assert not hl.grad.any()
+    with pytest.raises(IndexError):
+        linear_cross_entropy(h, w, torch.full_like(t, 50))
+
+
+def test_host_logic_on_emulated_kernels():
+    """Row compaction, upstream weights and reductions around the kernels, emulated on the CPU."""
+    from graspo_b200.ops.cross_entropy import _LinearCrossEntropy
+    from graspo_b200.ops.emulate import use_emulation
+
+    h, w, t, up = _case(150, 40, 333, 0.5, seed=2, device="cpu")
+    n = int((t != IGNORE).sum())
+    for reduction, scale in (("none", up), ("sum", torch.full_like(up, 0.5)), ("mean", torch.full_like(up, 0.5 / n))):
+        with use_emulation():
+            hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+            loss = _LinearCrossEntropy.apply(hl, wl, t, IGNORE, reduction, 256)
+            (loss * (up if reduction == "none" else 0.5)).sum().backward()
+        want, wh, ww, bound = _oracle(h, w, t, scale)
+        if reduction == "none":
+            _within(loss.detach(), want, bound["loss"], "loss")
+        _within(hl.grad, wh, bound["dh"], "dh")
+        _within(wl.grad, ww, bound["dw"], "dw")
+
+
+def test_refusals():
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy, linear_cross_entropy_grads
+
+    h, w, t = torch.randn(4, 8), torch.randn(10, 8), torch.zeros(4, dtype=torch.long)
+    for args, kw in [
+        ((h, w, t), {"reduction": "max"}),
+        ((h, w[:, :7], t), {}),
+        ((h, w[:0], t), {}),
+        ((h, w, t[:3]), {}),
+        ((h, w, t.float()), {}),
+        ((h, w[0], t), {}),
+    ]:
+        with pytest.raises(ValueError):
+            linear_cross_entropy(*args, **kw)
+    with pytest.raises(ValueError):
+        linear_cross_entropy_grads(h, w, t, grad=torch.ones(4))
+    with pytest.raises(ValueError):
+        linear_cross_entropy_grads(h, w, t, grad=torch.ones(3), reduction="none")
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy, linear_cross_entropy_grads
+
+    h, w, t, _ = _case(8, 64, 256, 1.0)
+    with pytest.raises(ValueError):
+        linear_cross_entropy(h.float(), w.float(), t)
+    with pytest.raises(ValueError):
+        linear_cross_entropy(h, w, t.cpu())
+    with pytest.raises(RuntimeError):
+        linear_cross_entropy_grads(h, w, t, piece=100)
