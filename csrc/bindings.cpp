@@ -100,15 +100,15 @@ void ce_scale(torch::Tensor token, torch::Tensor count, torch::Tensor grad, int6
 void ce_backward(torch::Tensor hc, torch::Tensor W, torch::Tensor place, torch::Tensor target, torch::Tensor count,
                  torch::Tensor lse, torch::Tensor scale, c10::optional<torch::Tensor> dh,
                  c10::optional<torch::Tensor> dW, int64_t piece, torch::Tensor err);
-void embed_fwd(torch::Tensor ids, torch::Tensor table, torch::Tensor y, double scale, torch::Tensor err);
-void embed_bwd(torch::Tensor dy, torch::Tensor ids, torch::Tensor out, double scale, int64_t padding, bool accumulate,
-               torch::Tensor err);
-void layer_norm_fwd(torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> b, torch::Tensor y,
-                    torch::Tensor mean, torch::Tensor rstd, double eps);
-void layer_norm_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w, torch::Tensor mean, torch::Tensor rstd,
-                    torch::Tensor dx, torch::Tensor dw, c10::optional<torch::Tensor> db);
-void grad_norm(std::vector<torch::Tensor> grads, torch::Tensor norm);
-void grad_clip(std::vector<torch::Tensor> grads, std::vector<torch::Tensor> out, double max_norm, torch::Tensor norm);
+torch::Tensor embed_fwd(torch::Tensor ids, torch::Tensor table, double scale, torch::Tensor err);
+torch::Tensor embed_bwd(torch::Tensor dy, torch::Tensor ids, int64_t vocab, c10::optional<torch::Tensor> into,
+                        double scale, int64_t padding, torch::Tensor err);
+std::vector<torch::Tensor> layer_norm_fwd(torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> b, double eps);
+std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w, torch::Tensor mean,
+                                          torch::Tensor rstd, bool bias32);
+torch::Tensor grad_norm(std::vector<torch::Tensor> grads, int64_t device);
+torch::Tensor grad_clip(std::vector<torch::Tensor> grads, std::vector<torch::Tensor> out, double max_norm,
+                        int64_t device);
 }  // namespace gb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -199,15 +199,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_backward", &gb::ce_backward, "gradients of the cross entropy, in pieces of the vocabulary", py::arg("hc"),
         py::arg("W"), py::arg("place"), py::arg("target"), py::arg("count"), py::arg("lse"), py::arg("scale"),
         py::arg("dh"), py::arg("dW"), py::arg("piece"), py::arg("err"));
-  m.def("embed_fwd", &gb::embed_fwd, "scaled embedding lookup", py::arg("ids"), py::arg("table"), py::arg("y"),
-        py::arg("scale"), py::arg("err"));
+  m.def("embed_fwd", &gb::embed_fwd, "scaled embedding lookup", py::arg("ids"), py::arg("table"), py::arg("scale"),
+        py::arg("err"));
   m.def("embed_bwd", &gb::embed_bwd, "gradient of the embedding table by sorted tokens", py::arg("dy"), py::arg("ids"),
-        py::arg("out"), py::arg("scale"), py::arg("padding"), py::arg("accumulate"), py::arg("err"));
+        py::arg("vocab"), py::arg("into"), py::arg("scale"), py::arg("padding"), py::arg("err"));
   m.def("layer_norm_fwd", &gb::layer_norm_fwd, "layer norm with its row statistics", py::arg("x"), py::arg("w"),
-        py::arg("b"), py::arg("y"), py::arg("mean"), py::arg("rstd"), py::arg("eps"));
+        py::arg("b"), py::arg("eps"));
   m.def("layer_norm_bwd", &gb::layer_norm_bwd, "gradients of layer norm for x, weight and bias", py::arg("dy"),
-        py::arg("x"), py::arg("w"), py::arg("mean"), py::arg("rstd"), py::arg("dx"), py::arg("dw"), py::arg("db"));
-  m.def("grad_norm", &gb::grad_norm, "global 2-norm of many tensors", py::arg("grads"), py::arg("norm"));
+        py::arg("x"), py::arg("w"), py::arg("mean"), py::arg("rstd"), py::arg("bias32"));
+  m.def("grad_norm", &gb::grad_norm, "global 2-norm of many tensors", py::arg("grads"),
+        py::arg("device"));
   m.def("grad_clip", &gb::grad_clip, "scale many tensors to a global 2-norm of at most max_norm", py::arg("grads"),
-        py::arg("out"), py::arg("max_norm"), py::arg("norm"));
+        py::arg("out"), py::arg("max_norm"), py::arg("device"));
 }

@@ -116,11 +116,9 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(const __nv_bfloat16* __r
     const bool live = m < n;
     const long src = !live ? 0 : token != nullptr ? token[m] : m;
     for (int c = threadIdx.x * V; c < ldo; c += blockDim.x * V) {
-      Pack<__nv_bfloat16, V> p;
-#pragma unroll
-      for (int i = 0; i < V; ++i) p.v[i] = __float2bfloat16(0.f);
-      if (live && c < H) p = *reinterpret_cast<const Pack<__nv_bfloat16, V>*>(in + src * ldi + c);
-      *reinterpret_cast<Pack<__nv_bfloat16, V>*>(out + m * ldo + c) = p;
+      Pack<__nv_bfloat16, V> p = {};
+      if (live && c < H) p = load_raw<__nv_bfloat16, V>(in + src * ldi + c);
+      store_raw<__nv_bfloat16, V>(out + m * ldo + c, p);
     }
   }
 }

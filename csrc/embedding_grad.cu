@@ -10,21 +10,27 @@
 // bf16, round at every addition.  The tokens are sorted by id instead (ties by
 // position), every row's tokens are then a run of the sorted list, and each run
 // is added in fp32 in token order and rounded once.
-//  * Sort: keys (id, position), sorted in shared memory 2048 at a time; a key's
-//    place in the whole is its place in its own chunk plus the number of smaller
-//    keys in every other chunk (a binary search each).  Two launches and no
+//  * Sort: 1024 tokens at a time, one per thread (bitonic; shuffles within a warp,
+//    shared memory across); a token's place in the whole is its place in its own
+//    chunk plus the number of smaller ids in every other chunk (a binary search
+//    each, the chunks shared out over a block's warps).  Two launches and no
 //    counters, for any number of tokens.
-//  * Long runs (one id over thousands of tokens, as padding makes them): whole
-//    groups of kGroup equal tokens are added first, all groups at once, and a run
-//    then adds those sums.
-//  * Rows: blocks take ranges of the table and find their tokens by binary
-//    search, so that every row is written once; or they take ranges of the
-//    sorted list when only touched rows are wanted.
+//  * Long runs (one id over thousands of tokens, as padding makes them): aligned
+//    groups of 32 equal tokens, and of 32 such groups, are added first, all at
+//    once, and a run then adds those sums: at most 62 tokens, 62 groups and its
+//    large groups one after the other.
+//  * Rows: a warp takes a few table rows and a slab of columns (neighbouring warps
+//    neighbouring slabs, so that blocks write contiguous memory), with every
+//    row's first place in the list at hand: every row is written once.  When only
+//    touched rows are wanted it takes a few places of the sorted list.  Few
+//    columns per warp rather than a block per row: most rows have no or one
+//    token, and what bounds them is the chain of dependent loads.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <stdexcept>
 
 #include "sm100_common.cuh"
 #include "vec_types.cuh"
@@ -33,379 +39,543 @@ namespace gb {
 
 namespace {
 
-constexpr int kSortKeys = 2048;       // keys per sorted chunk
-constexpr int kSortThreads = 1024;
-constexpr int kGroup = 32;            // tokens of a pre-added group
-constexpr int kRowThreads = 256;
-constexpr int kTableRows = 16;        // table rows per block
-constexpr int kListRows = 16;         // sorted positions per block
+constexpr int kSortKeys = 1024;       // tokens per sorted chunk, one per thread
+constexpr int kGroup = 32;            // tokens of a pre-added group, and groups of a large one
+constexpr int kGroupFrom = 128;       // tokens from which groups are worth their launch
+constexpr int kLargeFrom = 4096;      // ... and large groups theirs
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kTableRows = 8;         // table rows per warp
+constexpr int kListRows = 4;          // sorted places per warp
+constexpr int kLookup = 8;            // packs per thread of the lookup
 constexpr unsigned kNoId = 0xffffffffu;  // sorts last: no row takes it
+constexpr unsigned kAll = 0xffffffffu;
 
-using Key = unsigned long long;
+// Packs per lane of a slab, and rows of it in flight.
+template <int N>
+constexpr int kSlab = N == 1 ? 4 : 1;
+constexpr int kFlight = 8;       // tokens of a group: 32 registers of loads
+constexpr int kRunFlight = 4;    // tokens and sums of a run, where rows share the registers
 
 // y[t] = scale * table[id]; NaN for an id outside the table.  `lanes` threads a row.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kRowThreads) embed_fwd_kernel(const int64_t* __restrict__ ids, long T_, long V,
-                                                                const T* __restrict__ table, long ldt, int H,
-                                                                float scale, T* __restrict__ y, int lanes,
-                                                                int* __restrict__ err) {
+__global__ void __launch_bounds__(kThreads) embed_fwd_kernel(const int64_t* __restrict__ ids, long tokens, long V,
+                                                             const T* __restrict__ table, long ldt, int H, float scale,
+                                                             T* __restrict__ y, int lanes, int* __restrict__ err) {
   constexpr int N = kPackSize<T, WIDE>;
-  const int per_block = kRowThreads / lanes;
+  const int per_block = kThreads / lanes;
   const int lane = threadIdx.x % lanes;
   const int packs = H / N;
-  for (long t = blockIdx.x * static_cast<long>(per_block) + threadIdx.x / lanes; t < T_;
+  for (long t = blockIdx.x * static_cast<long>(per_block) + threadIdx.x / lanes; t < tokens;
        t += gridDim.x * static_cast<long>(per_block)) {
     const long id = ids[t];
     const bool ok = id >= 0 && id < V;
     if (!ok && lane == 0) atomicExch(err + 1, kErrBadToken);
-    const Pack<T, N>* src = reinterpret_cast<const Pack<T, N>*>(table + (ok ? id : 0) * ldt);
+    const T* src = table + (ok ? id : 0) * ldt;
     T* dst = y + t * H;
-#pragma unroll 4
-    for (int p = lane; p < packs; p += lanes) {
-      Pack<T, N> k;
-      if (ok) k = src[p];
-      float f[N];
+    for (int p0 = lane; p0 < packs; p0 += kLookup * lanes) {
+      Pack<T, N> k[kLookup];
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = ok ? to_f(k.v[i]) * scale : __int_as_float(0x7fc00000);
-      store_pack<T, N>(dst + static_cast<long>(p) * N, f);
-    }
-  }
-}
-
-// Sorted chunks of (id, position).  Padding ids, and ids outside the table
-// (reported), become kNoId.  With one chunk the result is final.
-__global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const int64_t* __restrict__ ids, long T, long V,
-                                                                  long padding, Key* __restrict__ keys,
-                                                                  unsigned* __restrict__ id_out,
-                                                                  int* __restrict__ token_out, bool final,
-                                                                  int* __restrict__ err) {
-  __shared__ Key s[kSortKeys];
-  const long base = static_cast<long>(blockIdx.x) * kSortKeys;
-  const int n = static_cast<int>(min(T - base, static_cast<long>(kSortKeys)));
-  int size = 2;
-  while (size < n) size <<= 1;
-  for (int i = threadIdx.x; i < size; i += kSortThreads) {
-    Key k = ~0ull;
-    if (i < n) {
-      const long id = ids[base + i];
-      unsigned u = static_cast<unsigned>(id);
-      if (id < 0 || id >= V) {
-        atomicExch(err + 1, kErrBadToken);
-        u = kNoId;
-      } else if (id == padding) {
-        u = kNoId;
-      }
-      k = static_cast<Key>(u) << 32 | static_cast<Key>(base + i);
-    }
-    s[i] = k;
-  }
-  __syncthreads();
-  for (int span = 2; span <= size; span <<= 1) {
-    for (int gap = span >> 1; gap > 0; gap >>= 1) {
-      for (int j = threadIdx.x; j < size >> 1; j += kSortThreads) {
-        const int i = (j / gap) * 2 * gap + j % gap;
-        const bool up = (i & span) == 0;
-        const Key a = s[i], b = s[i + gap];
-        if ((a > b) == up) {
-          s[i] = b;
-          s[i + gap] = a;
+      for (int u = 0; u < kLookup; ++u)
+        if (p0 + u * lanes < packs) k[u] = load_raw<T, N>(src + static_cast<long>(p0 + u * lanes) * N);
+#pragma unroll
+      for (int u = 0; u < kLookup; ++u)
+        if (p0 + u * lanes < packs) {
+          float f[N];
+#pragma unroll
+          for (int i = 0; i < N; ++i) f[i] = ok ? value(k[u], i) * scale : __int_as_float(0x7fc00000);
+          store_pack<T, N>(dst + static_cast<long>(p0 + u * lanes) * N, f);
         }
-      }
-      __syncthreads();
-    }
-  }
-  for (int i = threadIdx.x; i < n; i += kSortThreads) {
-    if (final) {
-      id_out[i] = static_cast<unsigned>(s[i] >> 32);
-      token_out[i] = static_cast<int>(s[i]);
-    } else {
-      keys[base + i] = s[i];
     }
   }
 }
 
-// Place of every key among all chunks.  Four chunks are searched side by side:
-// their loads do not wait for one another.
-__global__ void __launch_bounds__(256) embed_merge_kernel(const Key* __restrict__ keys, long T,
-                                                          unsigned* __restrict__ id_out, int* __restrict__ token_out) {
-  const long i = blockIdx.x * 256L + threadIdx.x;
-  if (i >= T) return;
-  const Key k = keys[i];
-  const int own = static_cast<int>(i / kSortKeys);
-  const int chunks = static_cast<int>((T + kSortKeys - 1) / kSortKeys);
-  long place = i - static_cast<long>(own) * kSortKeys;
-  for (int c0 = 0; c0 < chunks; c0 += 4) {
+// One step of the bitonic network on a key per thread: with the key `gap` threads
+// away, the lower thread of an ascending pair keeps the smaller one.
+template <int SPAN, int GAP, typename Key>
+__device__ __forceinline__ Key sort_step(Key k, Key (&s)[2][kSortKeys], int& flip) {
+  const int t = threadIdx.x;
+  Key other;
+  if constexpr (GAP >= 32) {
+    s[flip][t] = k;
+    __syncthreads();
+    other = s[flip][t ^ GAP];
+    flip ^= 1;  // the next step writes the other buffer: its readers are past this barrier
+  } else {
+    other = __shfl_xor_sync(kAll, k, GAP);
+  }
+  const bool keep_small = ((t & SPAN) == 0) == ((t & GAP) == 0);
+  k = keep_small ? min(k, other) : max(k, other);
+  if constexpr (GAP > 1) k = sort_step<SPAN, GAP / 2>(k, s, flip);
+  return k;
+}
+
+template <int SPAN, typename Key>
+__device__ __forceinline__ Key sort_keys(Key k, Key (&s)[2][kSortKeys], int& flip, int size) {
+  k = sort_step<SPAN, SPAN / 2>(k, s, flip);
+  if constexpr (SPAN < kSortKeys)
+    if (SPAN < size) k = sort_keys<2 * SPAN>(k, s, flip, size);
+  return k;
+}
+
+// Sorted chunks of (id, place in the chunk).  Padding ids, and ids outside the
+// table (reported), become the largest id, kNoId in the output.
+template <typename Key>
+__global__ void __launch_bounds__(kSortKeys) embed_sort_kernel(const int64_t* __restrict__ ids, long tokens, long V,
+                                                               long padding, unsigned* __restrict__ id_out,
+                                                               int* __restrict__ token_out, int* __restrict__ err) {
+  constexpr int kPlaceBits = 10;
+  constexpr Key kNone = ~Key(0) >> kPlaceBits;
+  static_assert(1 << kPlaceBits == kSortKeys, "a place fits its bits");
+  __shared__ Key s[2][kSortKeys];
+  const long base = static_cast<long>(blockIdx.x) * kSortKeys;
+  const int n = static_cast<int>(min(tokens - base, static_cast<long>(kSortKeys)));
+  const int t = threadIdx.x;
+  Key k = ~Key(0);  // past the end: after every token
+  if (t < n) {
+    const long id = ids[base + t];
+    Key u = kNone;
+    if (id < 0 || id >= V) atomicExch(err + 1, kErrBadToken);
+    else if (id != padding) u = static_cast<Key>(id);
+    k = u << kPlaceBits | static_cast<Key>(t);
+  }
+  int flip = 0;
+  k = sort_keys<2>(k, s, flip, n);  // the network of the next power of two
+  if (t < n) {
+    const Key id = k >> kPlaceBits;
+    id_out[base + t] = id == kNone ? kNoId : static_cast<unsigned>(id);
+    token_out[base + t] = static_cast<int>(base + static_cast<long>(k & (kSortKeys - 1)));
+  }
+}
+
+// Place of every token among all chunks: ids of earlier chunks come before equal
+// ids, those of later chunks after.  A block takes 32 tokens; its warps share out
+// the other chunks, four at a time, so that their loads do not wait for one another.
+__global__ void __launch_bounds__(kThreads) embed_merge_kernel(const unsigned* __restrict__ id,
+                                                               const int* __restrict__ token, int tokens,
+                                                               unsigned* __restrict__ id_out,
+                                                               int* __restrict__ token_out) {
+  __shared__ int before[kWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int i = blockIdx.x * 32 + lane;
+  const bool live = i < tokens;
+  const unsigned k = live ? id[i] : 0;
+  const int own = blockIdx.x * 32 / kSortKeys;
+  const int chunks = (tokens + kSortKeys - 1) / kSortKeys;
+  int place = 0;
+  for (int c0 = warp; c0 < chunks; c0 += 4 * kWarps) {
     int lo[4], n[4];
-    const Key* at[4];
+    const unsigned* at[4];
+    bool equal[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int c = c0 + u;
-      at[u] = keys + static_cast<long>(c) * kSortKeys;
-      n[u] = c < chunks && c != own ? static_cast<int>(min(T - static_cast<long>(c) * kSortKeys, static_cast<long>(kSortKeys))) : 0;
+      const int c = c0 + u * kWarps;
+      at[u] = id + static_cast<long>(c) * kSortKeys;
+      n[u] = live && c < chunks && c != own ? min(tokens - c * kSortKeys, kSortKeys) : 0;
+      equal[u] = c < own;
       lo[u] = 0;
     }
 #pragma unroll
     for (int step = kSortKeys; step > 0; step >>= 1) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (lo[u] + step <= n[u] && at[u][lo[u] + step - 1] < k) lo[u] += step;
+        if (lo[u] + step <= n[u]) {
+          const unsigned v = at[u][lo[u] + step - 1];
+          if (v < k || (equal[u] && v == k)) lo[u] += step;
+        }
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) place += lo[u];
   }
-  id_out[place] = static_cast<unsigned>(k >> 32);
-  token_out[place] = static_cast<int>(k);
+  before[warp][lane] = place;
+  __syncthreads();
+  if (warp == 0 && live) {
+    place = i - own * kSortKeys;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) place += before[w][lane];
+    id_out[place] = k;
+    token_out[place] = token[i];
+  }
 }
 
-// First position in [lo, hi) whose id is not below `id`; a whole warp calls it.
+// start[v] = first place of the sorted list whose id is not below v, v = 0 .. V.
+__global__ void __launch_bounds__(kThreads) embed_start_kernel(const unsigned* __restrict__ id, int tokens, int V,
+                                                               int* __restrict__ start) {
+  const int v = blockIdx.x * kThreads + threadIdx.x;
+  if (v > V) return;
+  int lo = 0, hi = tokens;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (id[mid] < static_cast<unsigned>(v)) lo = mid + 1;
+    else hi = mid;
+  }
+  start[v] = lo;
+}
+
+// First place in [lo, hi) whose id is not below `id`; a whole warp calls it.
 __device__ __forceinline__ int lower_bound_warp(const unsigned* __restrict__ ids, int lo, int hi, unsigned id) {
   const int lane = threadIdx.x & 31;
   while (hi - lo > 32) {
     const int step = (hi - lo + 32) / 33;
     const int at = lo + (lane + 1) * step - 1;
     const bool below = at < hi && ids[at] < id;
-    const int k = __popc(__ballot_sync(0xffffffffu, below));
+    const int k = __popc(__ballot_sync(kAll, below));
     hi = min(hi, lo + (k + 1) * step - (k < 32 ? 1 : 0));
     lo = lo + k * step;
   }
   const bool below = lo + lane < hi && ids[lo + lane] < id;
-  return lo + __popc(__ballot_sync(0xffffffffu, below));
-}
-
-template <int N>
-__device__ __forceinline__ void add_to(float (&acc)[N], const float (&f)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] += f[i];
-}
-
-// acc += dy[token[j]] at one pack, j = lo .. hi - 1 in order, eight loads in flight.
-template <typename T, int N>
-__device__ __forceinline__ void add_tokens(float (&acc)[N], const T* __restrict__ dy, long ld, int pack,
-                                           const int* __restrict__ token, int lo, int hi) {
-  int j = lo;
-  for (; j + 8 <= hi; j += 8) {
-    Pack<T, N> k[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) k[u] = reinterpret_cast<const Pack<T, N>*>(dy + token[j + u] * ld)[pack];
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += to_f(k[u].v[i]);
-  }
-  for (; j < hi; ++j) {
-    float f[N];
-    load_pack<T, N>(dy + token[j] * ld + static_cast<long>(pack) * N, f);
-    add_to(acc, f);
-  }
-}
-
-// Sums of the groups of kGroup sorted tokens that are all of one id.
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kRowThreads) embed_group_kernel(const T* __restrict__ dy, long ld, int H,
-                                                                  const unsigned* __restrict__ id,
-                                                                  const int* __restrict__ token, int ldg,
-                                                                  float* __restrict__ group) {
-  constexpr int N = kPackSize<T, WIDE>;
-  const int lo = blockIdx.x * kGroup;
-  if (id[lo] != id[lo + kGroup - 1] || id[lo] == kNoId) return;
-  const int packs = H / N;
-  for (int p = blockIdx.y * kRowThreads + threadIdx.x; p < packs; p += gridDim.y * kRowThreads) {
-    float acc[N] = {};
-    add_tokens<T, N>(acc, dy, ld, p, token, lo, lo + kGroup);
-#pragma unroll
-    for (int i = 0; i < N; ++i) group[static_cast<long>(blockIdx.x) * ldg + p * N + i] = acc[i];
-  }
-}
-
-// Sum of the run [a, b) at one pack: single tokens up to the first whole group,
-// the groups' sums, and the tokens after the last.
-template <typename T, int N>
-__device__ __forceinline__ void add_run(float (&acc)[N], const T* __restrict__ dy, long ld, int pack,
-                                        const int* __restrict__ token, const float* __restrict__ group, int ldg, int a,
-                                        int b) {
-  const int g0 = (a + kGroup - 1) / kGroup, g1 = b / kGroup;
-  if (g0 >= g1) {
-    add_tokens<T, N>(acc, dy, ld, pack, token, a, b);
-    return;
-  }
-  add_tokens<T, N>(acc, dy, ld, pack, token, a, g0 * kGroup);
-  for (int g = g0; g < g1; g += 8) {
-    float f[8][N];
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        f[u][i] = g + u < g1 ? group[static_cast<long>(g + u) * ldg + pack * N + i] : 0.f;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) add_to(acc, f[u]);
-  }
-  add_tokens<T, N>(acc, dy, ld, pack, token, g1 * kGroup, b);
+  return lo + __popc(__ballot_sync(kAll, below));
 }
 
 struct GradRows {
   const void* dy;
-  long ld;          // row stride of dy
-  const unsigned* id;
+  long ld;             // row stride of dy
+  const unsigned* id;  // sorted
   const int* token;
-  const float* group;
-  int ldg;
-  int T, V, H;
+  const float* group;  // [tokens / 32][ldg] sums of whole groups, null without them
+  const float* large;  // [tokens / 1024][ldg]
+  const int* start;    // [V + 1]; the whole table only
+  long ldg;
+  int tokens, V, H;
+  unsigned slabs;      // of columns
   float scale;
   void* out;
 };
 
-// The whole table: a block writes kTableRows rows, zeros where no token is.
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kRowThreads) embed_table_kernel(const GradRows g) {
-  constexpr int N = kPackSize<T, WIDE>;
-  __shared__ int bound[kTableRows + 1];
-  const int v0 = blockIdx.x * kTableRows;
-  const int rows = min(kTableRows, g.V - v0);
-  const int warp = threadIdx.x >> 5;
-  for (int i = warp; i <= rows; i += kRowThreads / 32) {
-    const int at = lower_bound_warp(g.id, 0, g.T, static_cast<unsigned>(v0 + i));
-    if ((threadIdx.x & 31) == 0) bound[i] = at;
-  }
-  __syncthreads();
-  const int packs = g.H / N;
-  for (int r = 0; r < rows; ++r) {
-    const int a = bound[r], b = bound[r + 1];
-    T* out = static_cast<T*>(g.out) + static_cast<long>(v0 + r) * g.H;
-    for (int p = blockIdx.y * kRowThreads + threadIdx.x; p < packs; p += gridDim.y * kRowThreads) {
-      float acc[N] = {};
-      if (a < b) {
-        add_run<T, N>(acc, static_cast<const T*>(g.dy), g.ld, p, g.token, g.group, g.ldg, a, b);
+// acc[s] += row(j) at pack p0 + 32 s, j = lo .. hi - 1 in order.  U rows are in
+// flight; `row` gives a row's address.
+template <typename T, int N, int S, int U, typename Row>
+__device__ __forceinline__ void add_rows(float (&acc)[S][N], int lo, int hi, int p0, int packs, Row&& row) {
+  int j = lo;
+#pragma unroll 1
+  for (; j + U <= hi; j += U) {
+    Pack<T, N> k[U][S];
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] *= g.scale;
-      }
-      store_pack<T, N>(out + static_cast<long>(p) * N, acc);
+    for (int u = 0; u < U; ++u) {
+      const T* src = row(j + u);
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (p0 + 32 * s < packs) k[u][s] = load_raw<T, N>(src + static_cast<long>(p0 + 32 * s) * N);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (p0 + 32 * s < packs)
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[s][i] += value(k[u][s], i);
+  }
+#pragma unroll 1
+  for (; j < hi; ++j) {
+    const T* src = row(j);
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (p0 + 32 * s < packs) {
+        const Pack<T, N> k = load_raw<T, N>(src + static_cast<long>(p0 + 32 * s) * N);
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[s][i] += value(k, i);
+      }
   }
 }
 
-// Adds to the touched rows of an existing gradient of type O: a block takes the
-// runs that start in its kListRows sorted positions.
-template <typename T, typename O, bool WIDE>
-__global__ void __launch_bounds__(kRowThreads) embed_list_kernel(const GradRows g) {
-  constexpr int N = kPackSize<T, WIDE>;
-  const int packs = g.H / N;
-  const int j0 = blockIdx.x * kListRows;
-  const int j1 = min(g.T, j0 + kListRows);
-  for (int j = j0; j < j1; ++j) {
-    const unsigned id = g.id[j];
-    if (id == kNoId) break;
-    if (j > 0 && g.id[j - 1] == id) continue;
-    const int end = lower_bound_warp(g.id, j, g.T, id + 1);
-    O* out = static_cast<O*>(g.out) + static_cast<long>(id) * g.H;
-    for (int p = blockIdx.y * kRowThreads + threadIdx.x; p < packs; p += gridDim.y * kRowThreads) {
-      float acc[N] = {}, old[N];
-      add_run<T, N>(acc, static_cast<const T*>(g.dy), g.ld, p, g.token, g.group, g.ldg, j, end);
-      load_pack<O, N>(out + static_cast<long>(p) * N, old);
+template <typename T, int U, int N, int S>
+__device__ __forceinline__ void add_tokens(float (&acc)[S][N], const GradRows& g, int lo, int hi, int p0, int packs) {
+  // 32 tokens' positions at once, one per lane
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int j0 = lo; j0 < hi; j0 += 32) {
+    const int mine = j0 + lane < hi ? g.token[j0 + lane] : 0;
+    add_rows<T, N, S, U>(acc, j0, min(hi, j0 + 32), p0, packs, [&](int j) {
+      return static_cast<const T*>(g.dy) + __shfl_sync(kAll, mine, j - j0) * g.ld;
+    });
+  }
+}
+
+template <int U, int N, int S>
+__device__ __forceinline__ void add_sums(float (&acc)[S][N], const float* sums, long ld, int lo, int hi, int p0,
+                                         int packs) {
+  add_rows<float, N, S, U>(acc, lo, hi, p0, packs, [&](int j) { return sums + j * ld; });
+}
+
+// A row's slab: scaled, added to what is there (ADD), and stored.
+template <typename O, bool ADD, int N, int S>
+__device__ __forceinline__ void store_row(const float (&acc)[S][N], float scale, O* out, int p0, int packs) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) old[i] += acc[i] * g.scale;
-      store_pack<O, N>(out + static_cast<long>(p) * N, old);
+  for (int s = 0; s < S; ++s)
+    if (p0 + 32 * s < packs) {
+      O* at = out + static_cast<long>(p0 + 32 * s) * N;
+      float f[N] = {};
+      if constexpr (ADD) load_pack<O, N>(at, f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] += acc[s][i] * scale;
+      store_pack<O, N>(at, f);
+    }
+}
+
+// A row with the run [a, b) of several tokens: tokens up to the first whole
+// group, groups up to the first large one, large groups, and back.  Kept out of
+// line, so that rows of none or one token need few registers.
+template <typename T, typename O, bool ADD, int N, int S>
+__device__ __noinline__ void run_row(const GradRows& g, int a, int b, int p0, int packs, O* out) {
+  float acc[S][N] = {};
+  const bool groups = g.group != nullptr && (a + kGroup - 1) / kGroup < b / kGroup;
+  const int ga = groups ? (a + kGroup - 1) / kGroup : 0, gb = groups ? b / kGroup : 0;
+  const bool larges = groups && g.large != nullptr && (ga + kGroup - 1) / kGroup < gb / kGroup;
+  const int la = larges ? (ga + kGroup - 1) / kGroup : 0, lb = larges ? gb / kGroup : 0;
+#pragma unroll 1
+  for (int part = 0; part < 5; ++part) {
+    if (part == 0 || part == 4) {
+      const int lo = part == 0 ? a : gb * kGroup, hi = part == 0 && groups ? ga * kGroup : b;
+      add_tokens<T, kRunFlight>(acc, g, lo, hi, p0, packs);
+      if (!groups) break;
+    } else {
+      const int lo = part == 1 ? ga : part == 2 ? la : larges ? lb * kGroup : gb;
+      const int hi = part == 2 ? lb : part == 1 && larges ? la * kGroup : gb;
+      add_sums<kRunFlight>(acc, part == 2 ? g.large : g.group, g.ldg, lo, hi, p0, packs);
     }
   }
+  store_row<O, ADD>(acc, g.scale, out, p0, packs);
+}
+
+// A row with the run [a, b), which may be empty.  The whole warp calls it.
+template <typename T, typename O, bool ADD, int N, int S>
+__device__ __forceinline__ void put_row(const GradRows& g, int a, int b, int p0, int packs, O* out) {
+  if (b - a > 1) {
+    run_row<T, O, ADD, N, S>(g, a, b, p0, packs, out);
+    return;
+  }
+  float acc[S][N] = {};
+  if (a < b) {
+    const T* src = static_cast<const T*>(g.dy) + g.token[a] * g.ld;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (p0 + 32 * s < packs) load_pack<T, N>(src + static_cast<long>(p0 + 32 * s) * N, acc[s]);
+  }
+  store_row<O, ADD>(acc, g.scale, out, p0, packs);
+}
+
+// A warp's work: its item (a group, some rows or places) and its first pack.
+// Neighbouring warps take neighbouring slabs of an item.
+struct WarpWork {
+  long item;
+  int pack;
+};
+
+template <int S>
+__device__ __forceinline__ WarpWork warp_work(const GradRows& g) {
+  const long w = blockIdx.x * static_cast<long>(kWarps) + (threadIdx.x >> 5);
+  const long item = w / g.slabs;
+  return {item, static_cast<int>(w - item * g.slabs) * 32 * S + static_cast<int>(threadIdx.x & 31)};
+}
+
+// Sums of the whole groups (LARGE: of the whole groups of groups) of one id.
+template <typename T, bool WIDE, bool LARGE>
+__global__ void __launch_bounds__(kThreads, 3) embed_group_kernel(const GradRows g, int groups, float* __restrict__ out) {
+  constexpr int N = kPackSize<T, WIDE>, S = kSlab<N>;
+  const WarpWork w = warp_work<S>(g);
+  if (w.item >= groups) return;
+  const int group = static_cast<int>(w.item), p0 = w.pack;
+  const int lo = group * (LARGE ? kGroup * kGroup : kGroup);
+  const unsigned id = g.id[lo];
+  if (id == kNoId || id != g.id[lo + (LARGE ? kGroup * kGroup : kGroup) - 1]) return;
+  const int packs = g.H / N;
+  float acc[S][N] = {};
+  if constexpr (LARGE) add_sums<kRunFlight>(acc, g.group, g.ldg, group * kGroup, (group + 1) * kGroup, p0, packs);
+  else add_tokens<T, kFlight>(acc, g, lo, lo + kGroup, p0, packs);
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (p0 + 32 * s < packs) store_pack<float, N>(out + group * g.ldg + static_cast<long>(p0 + 32 * s) * N, acc[s]);
+}
+
+// The whole table: a warp writes kTableRows rows' slabs, zeros where no token is.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 4) embed_table_kernel(const __grid_constant__ GradRows g) {
+  constexpr int N = kPackSize<T, WIDE>, S = kSlab<N>;
+  const int lane = threadIdx.x & 31;
+  const int packs = g.H / N;
+  const WarpWork w = warp_work<S>(g);
+  const long v0 = w.item * kTableRows;
+  if (v0 >= g.V) return;
+  const int rows = static_cast<int>(min(static_cast<long>(kTableRows), g.V - v0));
+  const int p0 = w.pack;
+  const int bound = lane <= rows ? g.start[v0 + lane] : 0;
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r) {
+    const int a = __shfl_sync(kAll, bound, r), b = __shfl_sync(kAll, bound, r + 1);
+    put_row<T, T, false, N, S>(g, a, b, p0, packs, static_cast<T*>(g.out) + (v0 + r) * g.H);
+  }
+}
+
+// Adds to the touched rows of an existing gradient of type O: a warp takes the
+// runs that start in its kListRows sorted places.
+template <typename T, typename O, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 4) embed_list_kernel(const __grid_constant__ GradRows g) {
+  constexpr int N = kPackSize<T, WIDE>, S = kSlab<N>;
+  const int lane = threadIdx.x & 31;
+  const int packs = g.H / N;
+  const WarpWork w = warp_work<S>(g);
+  if (w.item * kListRows >= g.tokens) return;
+  const int j0 = static_cast<int>(w.item) * kListRows, p0 = w.pack;
+  // ids of the places j0 - 1 .. j0 + 30
+  const int at = j0 - 1 + lane;
+  const unsigned near = at >= 0 && at < g.tokens ? g.id[at] : kNoId;
+#pragma unroll 1
+  for (int j = j0; j < min(g.tokens, j0 + kListRows); ++j) {
+    const unsigned id = __shfl_sync(kAll, near, j - j0 + 1);
+    if (id == kNoId) break;
+    if (j > 0 && __shfl_sync(kAll, near, j - j0) == id) continue;
+    // lanes from this place on that hold the id; up to the last lane: search on
+    const unsigned same = __ballot_sync(kAll, near == id && lane > j - j0);
+    int b = j + __popc(same);
+    if (same >> 31) b = lower_bound_warp(g.id, b, g.tokens, id + 1);
+    put_row<T, O, true, N, S>(g, j, b, p0, packs, static_cast<O*>(g.out) + static_cast<long>(id) * g.H);
+  }
+}
+
+// A ValueError in Python, as the CPU form's checks give.
+void require(bool ok, const char* what) {
+  if (!ok) throw std::invalid_argument(what);
+}
+
+torch::Tensor flat_ids(const torch::Tensor& ids, const torch::Tensor& like) {
+  require(ids.device() == like.device() && (ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32),
+          "ids must be int64 or int32 on the table's device");
+  const torch::Tensor wide = ids.scalar_type() == torch::kInt64 ? ids : ids.to(torch::kInt64);
+  return wide.contiguous();
+}
+
+unsigned blocks_for(long a, long b) {
+  const long n = (a + b - 1) / b;
+  require(n < (1L << 31), "sizes too large for one launch");
+  return static_cast<unsigned>(n);
 }
 
 }  // namespace
 
-void embed_fwd(torch::Tensor ids, torch::Tensor table, torch::Tensor y, double scale, torch::Tensor err) {
-  TORCH_CHECK(table.is_cuda() && is_storage_type(table) && table.dim() == 2 &&
-                  (table.stride(1) == 1 || table.size(1) == 1) && table.size(0) >= 1 && table.size(1) >= 1 &&
-                  table.size(1) < (1L << 31),
-              "table must be a bf16, fp16 or fp32 CUDA matrix with unit inner stride");
-  TORCH_CHECK(ids.device() == table.device() && ids.scalar_type() == torch::kInt64 && ids.is_contiguous(),
-              "ids must be contiguous int64 on the table's GPU");
-  TORCH_CHECK(y.device() == table.device() && y.scalar_type() == table.scalar_type() && y.is_contiguous() &&
-                  y.dim() == 2 && y.size(0) == ids.numel() && y.size(1) == table.size(1), "y must be [tokens, H] like the table");
+torch::Tensor embed_fwd(torch::Tensor ids, torch::Tensor table, double scale, torch::Tensor err) {
+  require(table.is_cuda() && is_storage_type(table) && table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1 &&
+              table.size(1) < (1L << 30),
+          "table must be a bf16, fp16 or fp32 CUDA matrix");
+  const torch::Tensor flat = flat_ids(ids, table);
   const c10::cuda::CUDAGuard guard(table.device());
-  const long T = ids.numel();
-  if (T == 0) return;
+  const torch::Tensor rows = table.stride(1) == 1 || table.size(1) == 1 ? table : table.contiguous();
+  const long tokens = flat.numel();
   const int H = static_cast<int>(table.size(1));
-  const bool wide = wide_rows(table) && wide_rows(y);
+  auto shape = ids.sizes().vec();
+  shape.push_back(H);
+  torch::Tensor y = torch::empty(shape, table.options());
+  if (tokens == 0) return y;
+  const bool wide = wide_rows(rows);
   by_type(table.scalar_type(), [&](auto tag) {
-    using E = decltype(tag);
-    const int packs = wide ? H / kPackSize<E, true> : H;
+    using T = decltype(tag);
+    const int packs = wide ? H / kPackSize<T, true> : H;
     int lanes = 32;
-    while (lanes < kRowThreads && lanes < packs) lanes <<= 1;
-    const long per_block = kRowThreads / lanes;
-    const unsigned blocks = static_cast<unsigned>(std::min<long>((T + per_block - 1) / per_block, 1L << 30));
-    (wide ? embed_fwd_kernel<E, true> : embed_fwd_kernel<E, false>)<<<blocks, kRowThreads, 0,
+    while (lanes < kThreads && lanes * kLookup < packs) lanes <<= 1;
+    const unsigned blocks = static_cast<unsigned>(std::min<long>(blocks_for(tokens, kThreads / lanes), 1L << 30));
+    (wide ? embed_fwd_kernel<T, true> : embed_fwd_kernel<T, false>)<<<blocks, kThreads, 0,
                                                                       at::cuda::getCurrentCUDAStream()>>>(
-        ids.data_ptr<int64_t>(), T, table.size(0), reinterpret_cast<const E*>(table.data_ptr()), table.stride(0), H,
-        static_cast<float>(scale), reinterpret_cast<E*>(y.data_ptr()), lanes, err.data_ptr<int>());
+        flat.data_ptr<int64_t>(), tokens, rows.size(0), reinterpret_cast<const T*>(rows.data_ptr()), rows.stride(0), H,
+        static_cast<float>(scale), reinterpret_cast<T*>(y.data_ptr()), lanes, err.data_ptr<int>());
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return y;
 }
 
-// dE [V, H]: written whole, or (accumulate) added to.  padding: an id without a gradient; one that no token has for none.
-void embed_bwd(torch::Tensor dy, torch::Tensor ids, torch::Tensor out, double scale, int64_t padding, bool accumulate,
-               torch::Tensor err) {
-  TORCH_CHECK(dy.is_cuda() && is_storage_type(dy) && dy.dim() == 2 && (dy.stride(1) == 1 || dy.size(1) == 1) &&
-                  dy.size(1) >= 1,
-              "dy must be a bf16, fp16 or fp32 CUDA matrix with unit inner stride");
-  TORCH_CHECK(ids.device() == dy.device() && ids.scalar_type() == torch::kInt64 && ids.is_contiguous() &&
-                  ids.numel() == dy.size(0), "ids must be contiguous int64, one per row of dy");
-  TORCH_CHECK(out.device() == dy.device() && is_storage_type(out) && out.is_contiguous() && out.dim() == 2 &&
-                  out.size(1) == dy.size(1) && out.size(0) >= 1, "the gradient must be a contiguous [V, H]");
-  TORCH_CHECK(accumulate || out.scalar_type() == dy.scalar_type(), "a gradient that is written whole has dy's type");
-  TORCH_CHECK(dy.size(0) < (1L << 31) - kSortKeys && out.size(0) < (1L << 31) - kTableRows && dy.size(1) < (1L << 31),
-              "sizes must fit 31 bits");
+// The gradient [vocab, H]: a new one of dy's type, or `out` added to.  padding: an
+// id without a gradient; one that no token has for none.
+torch::Tensor embed_bwd(torch::Tensor dy, torch::Tensor ids, int64_t vocab, c10::optional<torch::Tensor> into,
+                        double scale, int64_t padding, torch::Tensor err) {
+  require(dy.is_cuda() && is_storage_type(dy) && dy.dim() >= 1 && dy.size(-1) >= 1 && dy.size(-1) < (1L << 30),
+          "dy must be a bf16, fp16 or fp32 CUDA tensor [*ids.shape, H]");
+  const int64_t H = dy.size(-1), tokens = dy.numel() / H;
+  require(dy.sizes().slice(0, dy.dim() - 1) == ids.sizes(), "dy must have one row per id");
+  require(vocab >= 1 && vocab < (1L << 31) - kTableRows * kWarps && tokens < (1L << 31) - kSortKeys,
+          "the table needs a row, and sizes must fit 31 bits");
+  if (into.has_value())
+    require(into->device() == dy.device() && is_storage_type(*into) && into->is_contiguous() && into->dim() == 2 &&
+                into->size(0) == vocab && into->size(1) == H,
+            "out must be a contiguous bf16, fp16 or fp32 [vocab, H] on the device of dy");
+  const torch::Tensor flat = flat_ids(ids, dy);
   const c10::cuda::CUDAGuard guard(dy.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  const int T = static_cast<int>(dy.size(0)), H = static_cast<int>(dy.size(1)), V = static_cast<int>(out.size(0));
-  const int chunks = (T + kSortKeys - 1) / kSortKeys, groups = T / kGroup;
-  if (T == 0 && accumulate) return;
-  torch::Tensor ints = torch::empty({2, std::max(T, 1)}, dy.options().dtype(torch::kInt32));
-  unsigned* id = reinterpret_cast<unsigned*>(ints.data_ptr<int>());
-  int* token = ints.data_ptr<int>() + std::max(T, 1);
-  torch::Tensor keys, group;
-  if (chunks > 1) keys = torch::empty({T}, dy.options().dtype(torch::kInt64));
-  Key* k = chunks > 1 ? reinterpret_cast<Key*>(keys.data_ptr<int64_t>()) : nullptr;
-  if (T > 0) {
-    embed_sort_kernel<<<chunks, kSortThreads, 0, stream>>>(ids.data_ptr<int64_t>(), T, V, padding, k, id, token,
-                                                           chunks == 1, err.data_ptr<int>());
+  torch::Tensor out = into.has_value() ? *into : torch::empty({vocab, H}, dy.options());
+  if (tokens == 0) return into.has_value() ? out : out.zero_();
+  torch::Tensor rows = dy.reshape({tokens, H});
+  if (rows.stride(1) != 1 && H != 1) rows = rows.contiguous();
+
+  // sorted ids and tokens, the sorted chunks before their merge, and the rows' places
+  const bool one = tokens <= kSortKeys, whole = !into.has_value();
+  torch::Tensor ints = torch::empty({(one ? 2 : 4) * tokens + (whole ? vocab + 1 : 0)},
+                                    dy.options().dtype(torch::kInt32));
+  int* at = ints.data_ptr<int>();
+  unsigned* id = reinterpret_cast<unsigned*>(at);
+  int* token = at + tokens;
+  unsigned* id_chunks = one ? id : reinterpret_cast<unsigned*>(at + 2 * tokens);
+  int* token_chunks = one ? token : at + 3 * tokens;
+  int* start = at + (one ? 2 : 4) * tokens;
+  // 32-bit keys hold 10 bits of place and 22 of the id, whose last value is kept
+  (vocab < (1L << 22) ? embed_sort_kernel<unsigned> : embed_sort_kernel<unsigned long long>)<<<
+      blocks_for(tokens, kSortKeys), kSortKeys, 0, stream>>>(flat.data_ptr<int64_t>(), tokens, vocab, padding,
+                                                             id_chunks, token_chunks, err.data_ptr<int>());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (!one) {
+    embed_merge_kernel<<<blocks_for(tokens, 32), kThreads, 0, stream>>>(id_chunks, token_chunks,
+                                                                        static_cast<int>(tokens), id, token);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
-  if (chunks > 1) {
-    embed_merge_kernel<<<(T + 255) / 256, 256, 0, stream>>>(k, T, id, token);
+  if (whole) {
+    embed_start_kernel<<<blocks_for(vocab + 1, kThreads), kThreads, 0, stream>>>(id, static_cast<int>(tokens),
+                                                                                 static_cast<int>(vocab), start);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
-  const bool wide = wide_rows(dy) && aligned16(out.data_ptr()) && H * out.element_size() % 16 == 0;
+  const bool wide = wide_rows(rows) && aligned16(out.data_ptr()) && H * out.element_size() % 16 == 0;
   GradRows g{};
-  g.dy = dy.data_ptr();
-  g.ld = dy.stride(0);
+  g.dy = rows.data_ptr();
+  g.ld = rows.stride(0);
   g.id = id;
   g.token = token;
-  g.T = T, g.V = V, g.H = H;
+  g.start = start;
+  g.tokens = static_cast<int>(tokens), g.V = static_cast<int>(vocab), g.H = static_cast<int>(H);
   g.scale = static_cast<float>(scale);
   g.out = out.data_ptr();
+  torch::Tensor sums;
   by_type(dy.scalar_type(), [&](auto tag) {
-    using E = decltype(tag);
-    const int packs = wide ? H / kPackSize<E, true> : H;
-    const int columns = (packs + kRowThreads - 1) / kRowThreads;
-    if (groups > 0) {
-      g.ldg = static_cast<int>((H + 3) / 4 * 4);
-      group = torch::empty({groups, g.ldg}, dy.options().dtype(torch::kFloat32));
-      g.group = group.data_ptr<float>();
-      const dim3 grid(groups, std::min(columns, 8));
-      (wide ? embed_group_kernel<E, true> : embed_group_kernel<E, false>)<<<grid, kRowThreads, 0, stream>>>(
-          static_cast<const E*>(g.dy), g.ld, H, id, token, g.ldg, group.data_ptr<float>());
+    using T = decltype(tag);
+    const auto run = [&](auto wide_tag) {
+      constexpr bool W = decltype(wide_tag)::value;
+      constexpr int N = kPackSize<T, W>;
+      g.slabs = blocks_for(H / N, 32 * kSlab<N>);
+      if (tokens >= kGroupFrom) {
+        const long groups = tokens / kGroup, large = tokens >= kLargeFrom ? groups / kGroup : 0;
+        g.ldg = (H + 3) / 4 * 4;
+        sums = torch::empty({groups + large, g.ldg}, dy.options().dtype(torch::kFloat32));
+        float* group_sums = sums.data_ptr<float>();
+        embed_group_kernel<T, W, false><<<blocks_for(groups * g.slabs, kWarps), kThreads, 0, stream>>>(
+            g, static_cast<int>(groups), group_sums);
+        C10_CUDA_KERNEL_LAUNCH_CHECK();
+        g.group = group_sums;
+        if (large > 0) {
+          embed_group_kernel<T, W, true><<<blocks_for(large * g.slabs, kWarps), kThreads, 0, stream>>>(
+              g, static_cast<int>(large), group_sums + groups * g.ldg);
+          C10_CUDA_KERNEL_LAUNCH_CHECK();
+          g.large = group_sums + groups * g.ldg;
+        }
+      }
+      if (whole) {
+        embed_table_kernel<T, W>
+            <<<blocks_for(blocks_for(vocab, kTableRows) * static_cast<long>(g.slabs), kWarps), kThreads, 0, stream>>>(g);
+      } else {
+        by_type(out.scalar_type(), [&](auto otag) {
+          embed_list_kernel<T, decltype(otag), W>
+              <<<blocks_for(blocks_for(tokens, kListRows) * static_cast<long>(g.slabs), kWarps), kThreads, 0, stream>>>(g);
+        });
+      }
       C10_CUDA_KERNEL_LAUNCH_CHECK();
-    }
-    if (!accumulate) {
-      const dim3 grid((V + kTableRows - 1) / kTableRows, 1);
-      (wide ? embed_table_kernel<E, true> : embed_table_kernel<E, false>)<<<grid, kRowThreads, 0, stream>>>(g);
-    } else {
-      const dim3 grid((T + kListRows - 1) / kListRows, std::min(columns, 8));
-      by_type(out.scalar_type(), [&](auto otag) {
-        using O = decltype(otag);
-        (wide ? embed_list_kernel<E, O, true> : embed_list_kernel<E, O, false>)<<<grid, kRowThreads, 0, stream>>>(g);
-      });
-    }
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    };
+    if (wide) run(std::true_type{});
+    else run(std::false_type{});
   });
+  return out;
 }
 
 }  // namespace gb

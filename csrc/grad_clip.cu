@@ -6,14 +6,16 @@
 // where the tensors fit) and a write.  In place and below the limit the second
 // kernel returns after reading the norm.
 //
-// The tensors' addresses and sizes travel in the kernels' parameters, so a call
-// with some hundred tensors is two launches and copies no table to the GPU; no
-// address outlives the call.  The tensors are cut into chunks of kChunk values,
-// which blocks take in turn: the work is even however the sizes differ.  Each
-// block writes one double, and every block of the second kernel adds them in
-// the same order: the result does not depend on timing, and there is no counter
-// to reset.  Sums of squares are fp32 over at most some hundred values of one
-// thread, double from there on.
+// The tensors' addresses and sizes travel in the first kernel's parameters, so a
+// call with some hundred tensors copies no table to the GPU and is two launches;
+// the first kernel leaves the table in memory for the second.  No address
+// outlives the call.  The tensors are cut into chunks of kChunk values and every
+// block takes an equal stretch of them: the work is even however the sizes
+// differ, a block searches the table once, and runs through a large tensor in one
+// loop.  Each block writes one double, and
+// every block of the second kernel adds them in the same order: the result does
+// not depend on timing, and there is no counter to reset.  Sums of squares are
+// fp32 over the values that a thread loads at once, double from there on.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -29,9 +31,9 @@ namespace gb {
 
 namespace {
 
-constexpr int kChunk = 16384;        // values per chunk
+constexpr int kChunk = 4096;         // values; what the stretches are cut at
 constexpr int kClipThreads = 256;
-constexpr int kClipBlocks = 148 * 4;
+constexpr int kClipBlocks = 148 * 6;
 constexpr int kPerLaunch = 896;      // tensors per launch: the table stays below the 32 KB of kernel parameters
 
 enum GradType : uint8_t { kF32 = 0, kBF16 = 1, kF16 = 2 };
@@ -49,18 +51,25 @@ struct GradTable {
   GradEntry e[N];
   int tensors;
   int chunks;      // in all
+  int at;          // place of entry 0 in the whole table, and
+  int first;       // of chunk 0 among all chunks
 };
 
 // Entry of chunk c: the last one whose first chunk is not past it.
-template <int N>
-__device__ __forceinline__ int entry_of(const GradTable<N>& t, int c) {
-  int lo = 0, hi = t.tensors;
+__device__ __forceinline__ int entry_of(const GradEntry* e, int tensors, int c) {
+  int lo = 0, hi = tensors;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (t.e[mid].first <= c) lo = mid;
+    if (e[mid].first <= c) lo = mid;
     else hi = mid;
   }
   return lo;
+}
+
+// Stretch [begin, end) of `chunks` that a block takes.
+__device__ __forceinline__ int2 stretch(int chunks) {
+  return make_int2(static_cast<int>(static_cast<long>(chunks) * blockIdx.x / gridDim.x),
+                   static_cast<int>(static_cast<long>(chunks) * (blockIdx.x + 1) / gridDim.x));
 }
 
 template <typename F>
@@ -70,30 +79,39 @@ __device__ __forceinline__ void by_grad_type(uint8_t type, F&& f) {
   else f(static_cast<__half*>(nullptr));
 }
 
-// Sum of squares of values [lo, hi) of g: 16-byte loads, four in flight per thread,
-// between the values before the first and after the last 16-byte boundary.
+// Sum of squares of this thread's values among [lo, hi) of g: 16-byte loads, four
+// in flight, between the values before the first and after the last 16-byte
+// boundary; fp32 over one round of loads, double across rounds.
 template <typename T>
-__device__ __forceinline__ float sumsq_range(const T* g, long lo, long hi) {
-  constexpr int V = 16 / sizeof(T);
+__device__ __noinline__ double sumsq_range(const T* __restrict__ g, long lo, long hi) {
+  constexpr int V = 16 / sizeof(T), U = 4;
   const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(g + lo) & 15) / sizeof(T));
   const long a = min(hi, lo + (skew == 0 ? 0 : V - skew));
   const long packs = (hi - a) / V;
-  float s[4] = {};
-  for (long i = lo + threadIdx.x; i < a; i += kClipThreads) s[0] += to_f(g[i]) * to_f(g[i]);
-  for (long i = a + packs * V + threadIdx.x; i < hi; i += kClipThreads) s[1] += to_f(g[i]) * to_f(g[i]);
   const T* body = g + a;
-  for (long p = threadIdx.x; p < packs; p += 4 * kClipThreads) {
-    Pack<T, V> k[4];
+  double total = 0;
+  long p = threadIdx.x;
+  for (; p + (U - 1) * kClipThreads < packs; p += U * kClipThreads) {
+    Pack<T, V> k[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (p + u * kClipThreads < packs) k[u] = reinterpret_cast<const Pack<T, V>*>(body)[p + u * kClipThreads];
+    for (int u = 0; u < U; ++u) k[u] = load_raw<T, V>(body + (p + u * kClipThreads) * V);
+    float s[U] = {};
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (p + u * kClipThreads < packs)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[u] += to_f(k[u].v[i]) * to_f(k[u].v[i]);
+      for (int i = 0; i < V; ++i) s[u] += value(k[u], i) * value(k[u], i);
+    total += (s[0] + s[1]) + (s[2] + s[3]);
   }
-  return (s[0] + s[1]) + (s[2] + s[3]);
+  float s = 0.f;
+  for (; p < packs; p += kClipThreads) {
+    const Pack<T, V> k = load_raw<T, V>(body + p * V);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s += value(k, i) * value(k, i);
+  }
+  if (lo + threadIdx.x < a) s += to_f(g[lo + threadIdx.x]) * to_f(g[lo + threadIdx.x]);
+  const long tail = a + packs * V + threadIdx.x;
+  if (tail < hi) s += to_f(g[tail]) * to_f(g[tail]);
+  return total + s;
 }
 
 __device__ __forceinline__ double block_sum(double v) {
@@ -109,18 +127,31 @@ __device__ __forceinline__ double block_sum(double v) {
   return v;
 }
 
+// `table`: the whole call's entries for the second kernel, null without one.
 template <int N>
-__global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const __grid_constant__ GradTable<N> t,
+__global__ void __launch_bounds__(kClipThreads, 6) grad_norm_kernel(const __grid_constant__ GradTable<N> t,
+                                                                 GradEntry* __restrict__ table,
                                                                  double* __restrict__ partial) {
+  if (table != nullptr && blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < t.tensors; i += kClipThreads) {
+      GradEntry e = t.e[i];
+      e.first += t.first;
+      table[t.at + i] = e;
+    }
+  }
   double total = 0;
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    const GradEntry& e = t.e[entry_of(t, c)];
+  const int2 own = stretch(t.chunks);
+  int i = entry_of(t.e, t.tensors, own.x);
+  for (int c = own.x; c < own.y; ++i) {
+    const GradEntry& e = t.e[i];
+    const int past = i + 1 < t.tensors ? min(own.y, t.e[i + 1].first) : own.y;
     const long lo = static_cast<long>(c - e.first) * kChunk;
-    const long hi = min(e.n, lo + kChunk);
+    const long hi = min(e.n, static_cast<long>(past - e.first) * kChunk);
     by_grad_type(e.tin, [&](auto* tag) {
       using T = std::remove_pointer_t<decltype(tag)>;
       total += sumsq_range(static_cast<const T*>(e.in), lo, hi);
     });
+    c = past;
   }
   total = block_sum(total);
   if (threadIdx.x == 0) partial[blockIdx.x] = total;
@@ -141,34 +172,43 @@ __global__ void __launch_bounds__(kClipThreads) grad_norm_finish_kernel(const do
 // out = coef * in over [lo, hi).  16-byte accesses where the input and the output
 // reach their boundaries at the same value, single values elsewhere.
 template <typename T, typename O>
-__device__ __forceinline__ void scale_range(const T* g, O* out, long lo, long hi, float coef) {
-  constexpr int V = 8, W = 16 / sizeof(T);
-  const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(g + lo) & 15) / sizeof(T));
-  long a = min(hi, lo + (skew == 0 ? 0 : W - skew));
-  if ((reinterpret_cast<uintptr_t>(out + a) & 15) != 0) a = hi;
+__device__ __noinline__ void scale_range(const T* g, O* out, long lo, long hi, float coef) {
+  // a warp's accesses of the wider type are 512 contiguous bytes
+  constexpr int V = 16 / static_cast<int>(sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
+  constexpr int A = V * static_cast<int>(sizeof(T)), B = V * static_cast<int>(sizeof(O));
+  const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(g + lo) & (A - 1)) / sizeof(T));
+  long a = min(hi, lo + (skew == 0 ? 0 : V - skew));
+  if ((reinterpret_cast<uintptr_t>(out + a) & (B - 1)) != 0) a = hi;
   const long packs = (hi - a) / V;
   for (long i = lo + threadIdx.x; i < a; i += kClipThreads) out[i] = from_f<O>(to_f(g[i]) * coef);
   for (long i = a + packs * V + threadIdx.x; i < hi; i += kClipThreads) out[i] = from_f<O>(to_f(g[i]) * coef);
-  for (long p = threadIdx.x; p < packs; p += 2 * kClipThreads) {
-    float f[2][V];
+  constexpr int U = 4;
+  const long rounds = packs / (U * kClipThreads);
+  for (long p = rounds * U * kClipThreads + threadIdx.x; p < packs; p += kClipThreads) {
+    float f[V];
+    load_pack<T, V>(g + a + p * V, f);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (p + u * kClipThreads < packs) load_pack<T, V>(g + a + (p + u * kClipThreads) * V, f[u]);
+    for (int i = 0; i < V; ++i) f[i] *= coef;
+    store_pack<O, V>(out + a + p * V, f);
+  }
+  for (long p = (rounds - 1) * U * kClipThreads + threadIdx.x; p >= 0; p -= U * kClipThreads) {
+    Pack<T, V> k[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (p + u * kClipThreads < packs) {
+    for (int u = 0; u < U; ++u) k[u] = load_raw<T, V>(g + a + (p + u * kClipThreads) * V);
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[u][i] *= coef;
-        store_pack<O, V>(out + a + (p + u * kClipThreads) * V, f[u]);
-      }
+    for (int u = 0; u < U; ++u) {
+      float f[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = value(k[u], i) * coef;
+      store_pack<O, V>(out + a + (p + u * kClipThreads) * V, f);
+    }
   }
 }
 
 // `in_place`: every output is its input, so a coefficient of 1 leaves nothing to do.
-template <int N>
-__global__ void __launch_bounds__(kClipThreads) grad_scale_kernel(const __grid_constant__ GradTable<N> t,
-                                                                  const double* __restrict__ partial, int count,
-                                                                  float max_norm, bool in_place,
+__global__ void __launch_bounds__(kClipThreads, 4) grad_scale_kernel(const GradEntry* __restrict__ table, int tensors,
+                                                                  int chunks, const double* __restrict__ partial,
+                                                                  int count, float max_norm, bool in_place,
                                                                   float* __restrict__ norm) {
   const float n = norm_of(partial, count);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
@@ -178,11 +218,14 @@ __global__ void __launch_bounds__(kClipThreads) grad_scale_kernel(const __grid_c
     coef = q > 1.f ? 1.f : q;  // a NaN norm stays one
   }
   if (in_place && coef == 1.f) return;
-  // from the end: the norm's walk read those values last
-  for (int c = t.chunks - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= gridDim.x) {
-    const GradEntry& e = t.e[entry_of(t, c)];
+  // backwards: the norm's walk read the ends of the stretches last, and they may still be in L2
+  const int2 own = stretch(chunks);
+  int i = entry_of(table, tensors, own.y - 1);
+  for (int past = own.y; past > own.x; --i) {
+    const GradEntry e = table[i];
+    const int c = max(own.x, e.first);
     const long lo = static_cast<long>(c - e.first) * kChunk;
-    const long hi = min(e.n, lo + kChunk);
+    const long hi = min(e.n, static_cast<long>(past - e.first) * kChunk);
     by_grad_type(e.tin, [&](auto* tag) {
       using T = std::remove_pointer_t<decltype(tag)>;
       by_grad_type(e.tout, [&](auto* otag) {
@@ -190,6 +233,7 @@ __global__ void __launch_bounds__(kClipThreads) grad_scale_kernel(const __grid_c
         scale_range(static_cast<const T*>(e.in), static_cast<O*>(e.out), lo, hi, coef);
       });
     });
+    past = c;
   }
 }
 
@@ -207,22 +251,23 @@ void require(bool ok, const char* what) {
   if (!ok) throw std::invalid_argument(what);
 }
 
-// Entries of the tensors that hold values; chunks counted per launch.
+// Entries of the tensors that hold values.
 std::vector<GradEntry> entries(const std::vector<torch::Tensor>& in, const std::vector<torch::Tensor>* out,
                                const torch::Tensor& like) {
   std::vector<GradEntry> v;
   v.reserve(in.size());
+  const auto device = like.device();
   for (size_t i = 0; i < in.size(); ++i) {
     const torch::Tensor& t = in[i];
-    require(t.device() == like.device() && t.is_contiguous(), "gradients must be contiguous and on one device");
+    require(t.device() == device && t.is_contiguous(), "gradients must be contiguous and on one device");
     GradEntry e{};
     e.in = t.data_ptr();
     e.n = t.numel();
     e.tin = e.tout = grad_type(t);
-    e.out = t.data_ptr();
+    e.out = const_cast<void*>(e.in);
     if (out != nullptr) {
       const torch::Tensor& o = (*out)[i];
-      require(o.device() == like.device() && o.is_contiguous() && o.sizes() == t.sizes(),
+      require(o.device() == device && o.is_contiguous() && o.sizes() == t.sizes(),
               "outputs must be contiguous, on the gradients' device and of their shapes");
       e.out = o.data_ptr();
       e.tout = grad_type(o);
@@ -232,83 +277,96 @@ std::vector<GradEntry> entries(const std::vector<torch::Tensor>& in, const std::
   return v;
 }
 
-template <typename F>
-void for_tables(const std::vector<GradEntry>& v, F&& launch) {
-  const auto fill = [&](auto& table, size_t from, size_t count) {
+// The norm's launches: sums of squares of all tensors, one double per block.
+struct NormPass {
+  torch::Tensor buffer;       // doubles, then the table
+  const double* partial;
+  int count = 0;              // doubles
+  const GradEntry* table;     // filled when asked for
+  int tensors, chunks = 0;
+};
+
+NormPass norm_pass(const std::vector<GradEntry>& v, bool want_table, const torch::Tensor& like, cudaStream_t stream) {
+  NormPass r;
+  const size_t launches = std::max<size_t>((v.size() + kPerLaunch - 1) / kPerLaunch, 1);
+  const int64_t doubles = static_cast<int64_t>(launches) * kClipBlocks;
+  r.buffer = torch::empty({doubles * 8 + static_cast<int64_t>(want_table ? v.size() * sizeof(GradEntry) : 0)},
+                          like.options().dtype(torch::kUInt8));
+  double* partial = reinterpret_cast<double*>(r.buffer.data_ptr());
+  GradEntry* table = want_table ? reinterpret_cast<GradEntry*>(partial + doubles) : nullptr;
+  r.partial = partial;
+  r.table = table;
+  r.tensors = static_cast<int>(v.size());
+  long chunks_before = 0;
+  const auto run = [&](auto& t, size_t from, size_t count) {
     long chunks = 0;
     for (size_t i = 0; i < count; ++i) {
-      table.e[i] = v[from + i];
-      table.e[i].first = static_cast<int>(chunks);
+      t.e[i] = v[from + i];
+      t.e[i].first = static_cast<int>(chunks);
       chunks += (v[from + i].n + kChunk - 1) / kChunk;
+      require(chunks_before + chunks < (1L << 31) - kClipBlocks, "gradients too large for one call");
     }
-    require(chunks < (1L << 31) - kClipBlocks, "gradients too large for one call");
-    table.tensors = static_cast<int>(count);
-    table.chunks = static_cast<int>(chunks);
+    t.tensors = static_cast<int>(count);
+    t.chunks = static_cast<int>(chunks);
+    t.at = static_cast<int>(from);
+    t.first = static_cast<int>(chunks_before);
+    const int blocks = static_cast<int>(std::min<long>(chunks, kClipBlocks));
+    grad_norm_kernel<<<blocks, kClipThreads, 0, stream>>>(t, table, partial + r.count);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    r.count += blocks;
+    chunks_before += chunks;
   };
   for (size_t from = 0; from < v.size(); from += kPerLaunch) {
     const size_t count = std::min<size_t>(kPerLaunch, v.size() - from);
-    if (count <= 64) {  // 2 KB of parameters instead of 32
-      GradTable<64> table;
-      fill(table, from, count);
-      launch(table);
+    if (count <= 64) {  // 2 KB of parameters instead of 28
+      GradTable<64> t;
+      run(t, from, count);
     } else {
-      GradTable<kPerLaunch> table;
-      fill(table, from, count);
-      launch(table);
+      GradTable<kPerLaunch> t;
+      run(t, from, count);
     }
   }
+  r.chunks = static_cast<int>(chunks_before);
+  return r;
 }
 
-int table_blocks(int chunks) { return std::min(chunks, kClipBlocks); }
-
-// Sums of squares of all tensors: one double per block, every launch its own range.
-torch::Tensor norm_partials(const std::vector<GradEntry>& v, const torch::Tensor& like, cudaStream_t stream,
-                            int* count) {
-  const int launches = static_cast<int>((v.size() + kPerLaunch - 1) / kPerLaunch);
-  torch::Tensor partial = torch::empty({std::max(launches, 1) * kClipBlocks}, like.options().dtype(torch::kFloat64));
-  int at = 0;
-  for_tables(v, [&](auto& table) {
-    const int blocks = table_blocks(table.chunks);
-    grad_norm_kernel<<<blocks, kClipThreads, 0, stream>>>(table, partial.data_ptr<double>() + at);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-    at += blocks;
-  });
-  *count = at;
-  return partial;
+torch::Tensor norm_on(int64_t device) {
+  require(device >= 0, "a CUDA device");
+  return torch::empty({}, torch::TensorOptions().dtype(torch::kFloat32).device(torch::kCUDA, static_cast<c10::DeviceIndex>(device)));
 }
 
 }  // namespace
 
-void grad_norm(std::vector<torch::Tensor> grads, torch::Tensor norm) {
-  TORCH_CHECK(norm.is_cuda() && norm.scalar_type() == torch::kFloat32 && norm.numel() == 1, "norm must be one CUDA fp32 value");
+// 2-norm of all values; `device` where there are no tensors to tell it.
+torch::Tensor grad_norm(std::vector<torch::Tensor> grads, int64_t device) {
+  torch::Tensor norm = norm_on(device);
   const c10::cuda::CUDAGuard guard(norm.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  int count = 0;
-  const torch::Tensor partial = norm_partials(entries(grads, nullptr, norm), norm, stream, &count);
-  grad_norm_finish_kernel<<<1, kClipThreads, 0, stream>>>(partial.data_ptr<double>(), count, norm.data_ptr<float>());
+  const NormPass r = norm_pass(entries(grads, nullptr, norm), false, norm, stream);
+  grad_norm_finish_kernel<<<1, kClipThreads, 0, stream>>>(r.partial, r.count, norm.data_ptr<float>());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return norm;
 }
 
 // out: empty to scale the gradients in place.
-void grad_clip(std::vector<torch::Tensor> grads, std::vector<torch::Tensor> out, double max_norm, torch::Tensor norm) {
-  TORCH_CHECK(norm.is_cuda() && norm.scalar_type() == torch::kFloat32 && norm.numel() == 1, "norm must be one CUDA fp32 value");
+torch::Tensor grad_clip(std::vector<torch::Tensor> grads, std::vector<torch::Tensor> out, double max_norm,
+                        int64_t device) {
   require(out.empty() || out.size() == grads.size(), "one output per gradient");
   require(max_norm >= 0, "max_norm must not be negative");
+  torch::Tensor norm = norm_on(device);
   const c10::cuda::CUDAGuard guard(norm.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool in_place = out.empty();
-  const std::vector<GradEntry> v = entries(grads, in_place ? nullptr : &out, norm);
-  int count = 0;
-  const torch::Tensor partial = norm_partials(v, norm, stream, &count);
-  if (v.empty()) {
-    grad_norm_finish_kernel<<<1, kClipThreads, 0, stream>>>(partial.data_ptr<double>(), 0, norm.data_ptr<float>());
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-  }
-  for_tables(v, [&](auto& table) {
-    grad_scale_kernel<<<table_blocks(table.chunks), kClipThreads, 0, stream>>>(
-        table, partial.data_ptr<double>(), count, static_cast<float>(max_norm), in_place, norm.data_ptr<float>());
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-  });
+  const NormPass r = norm_pass(entries(grads, in_place ? nullptr : &out, norm), true, norm, stream);
+  const int blocks = std::max(1, std::min(r.chunks, kClipBlocks));
+  if (r.tensors > 0)
+    grad_scale_kernel<<<blocks, kClipThreads, 0, stream>>>(r.table, r.tensors, r.chunks, r.partial, r.count,
+                                                           static_cast<float>(max_norm), in_place,
+                                                           norm.data_ptr<float>());
+  else
+    grad_norm_finish_kernel<<<1, kClipThreads, 0, stream>>>(r.partial, 0, norm.data_ptr<float>());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return norm;
 }
 
 }  // namespace gb

@@ -6,21 +6,28 @@
 //   dw = sum_rows dy n,  db = sum_rows dy                   per column
 //
 // Memory bound: the forward reads x and writes y, the backward reads x and dy
-// and writes dx.  A row is read once and kept in registers, where the mean and
-// then the centred sum of squares are taken (fp32; no cancellation of
-// E[x^2] - mean^2).  A thread meets the same columns in every row that its
-// block walks, so it carries its columns' dw and db in registers; the blocks'
-// sums are joined by a second, small kernel in a fixed order.
+// and writes dx.
 //
-// Variants: up to 160 packs of 16 bytes a row (1280 bf16 values) take a warp a
-// row, several rows per block and no barrier; longer ones a block a row; rows
-// past 2048 packs are read several times (they stay in L1/L2).  Rows that are no
-// multiple of 16 bytes are read value by value.
+// Forward: a row is read once and kept in registers, where the mean and then the
+// centred sum of squares are taken (fp32; no cancellation of E[x^2] - mean^2).
+// Up to 1280 bf16 values a warp takes a row: no barrier, many rows in flight.
+//
+// Backward: besides a row's two sums there are two sums per column.  A thread
+// owns a few columns for all rows of its block, so that those stay in registers,
+// and takes R rows at a time: their loads are in flight together and their 2 R
+// row sums share two barriers.  (A warp a row needs 80 registers of column sums
+// a thread at 1152 columns and left one block of 256 threads per SM.)  Rows of
+// up to 64 packs keep the warp-a-row form.  The blocks' column sums are joined
+// by a second, small kernel in a fixed order.
+//
+// Rows that are no multiple of 16 bytes are read value by value; rows past the
+// variants below are walked several times (they stay in L1/L2).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <stdexcept>
 
 #include "sm100_common.cuh"
 #include "vec_types.cuh"
@@ -65,6 +72,27 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* scratch) {
   return make_float2(a, b);
 }
 
+// Sums of N values over the warp (N a power of two, at most 32): each step
+// exchanges half of the values, so that N - 1 + 5 - log2 N shuffles do it rather
+// than 5 N.  Lane l gets the sum of value l >> (5 - log2 N).
+template <int N>
+__device__ __forceinline__ float warp_sum_many(float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  int bit = 16;
+#pragma unroll
+  for (int half = N / 2; half > 0; half >>= 1) {
+    const bool up = (lane & bit) != 0;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float give = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+    }
+    bit >>= 1;
+  }
+  for (; bit > 0; bit >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);
+  return v[0];
+}
+
 // weight / bias values: fp32, or the type of x
 template <typename T, int V>
 __device__ __forceinline__ void load_param(const void* p, bool fp32, long i, float (&f)[V]) {
@@ -101,7 +129,7 @@ struct NormArgs {
 };
 
 template <typename T, int V, int VPT, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kWarpRows) ln_fwd_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kWarpRows, BLOCK ? 1 : 3) ln_fwd_kernel(const NormArgs a) {
   __shared__ float scratch[32];
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31;
   const int width = BLOCK ? blockDim.x : 32;
@@ -114,13 +142,13 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kWarpRows) ln_fwd_kernel(co
     Pack<T, V> raw[VPT];
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
-      if (lane + k * width < packs) raw[k] = reinterpret_cast<const Pack<T, V>*>(x)[lane + k * width];
+      if (lane + k * width < packs) raw[k] = load_raw<T, V>(x + static_cast<long>(lane + k * width) * V);
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
       if (lane + k * width < packs)
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += to_f(raw[k].v[i]);
+        for (int i = 0; i < V; ++i) s += value(raw[k], i);
     const float mean = row_sum<BLOCK>(s, scratch) * inv_h;
     s = 0.f;
 #pragma unroll
@@ -128,7 +156,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kWarpRows) ln_fwd_kernel(co
       if (lane + k * width < packs)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float c = to_f(raw[k].v[i]) - mean;
+          const float c = value(raw[k], i) - mean;
           s += c * c;
         }
     const float rstd = 1.f / sqrtf(row_sum<BLOCK>(s, scratch) * inv_h + a.eps);
@@ -141,8 +169,84 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kWarpRows) ln_fwd_kernel(co
         load_param<T, V>(a.w, a.w32, static_cast<long>(p) * V, w);
         if (a.b != nullptr) load_param<T, V>(a.b, a.b32, static_cast<long>(p) * V, b);
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = (to_f(raw[k].v[i]) - mean) * rstd * w[i] + b[i];
+        for (int i = 0; i < V; ++i) o[i] = (value(raw[k], i) - mean) * rstd * w[i] + b[i];
         store_pack<T, V>(y + static_cast<long>(p) * V, o);
+      }
+    }
+    if (lane == 0) {
+      a.mean[r] = mean;
+      a.rstd[r] = rstd;
+    }
+  }
+}
+
+// The warp-a-row forward for many rows: blocks stay, weight and bias wait in
+// shared memory as fp32 (unpacking them for every row was a quarter of the
+// instructions), and a warp's next row is on its way while it works on one.
+template <typename T, int V, int VPT>
+__global__ void __launch_bounds__(32 * kWarpRows, 3) ln_fwd_many_kernel(const NormArgs a) {
+  static_assert(V % 4 == 0, "whole float4");
+  __shared__ float4 param[2][VPT * (V / 4)][32];  // [weight, bias][pack and quarter][lane]
+  const int lane = threadIdx.x & 31;
+  const int packs = a.H / V;
+  const float inv_h = 1.f / static_cast<float>(a.H);
+  for (int p = threadIdx.x; p < packs; p += blockDim.x) {
+    float w[V], b[V] = {};
+    load_param<T, V>(a.w, a.w32, static_cast<long>(p) * V, w);
+    if (a.b != nullptr) load_param<T, V>(a.b, a.b32, static_cast<long>(p) * V, b);
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      param[0][(p >> 5) * (V / 4) + q][p & 31] = make_float4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+      param[1][(p >> 5) * (V / 4) + q][p & 31] = make_float4(b[4 * q], b[4 * q + 1], b[4 * q + 2], b[4 * q + 3]);
+    }
+  }
+  __syncthreads();
+  const long step = gridDim.x * static_cast<long>(kWarpRows);
+  long r = blockIdx.x * static_cast<long>(kWarpRows) + (threadIdx.x >> 5);
+  Pack<T, V> next[VPT];
+  const auto fetch = [&](long row) {
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+      if (lane + k * 32 < packs) next[k] = load_raw<T, V>(x + (lane + k * 32) * V);
+  };
+  if (r < a.rows) fetch(r);
+  for (; r < a.rows; r += step) {
+    Pack<T, V> raw[VPT];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) raw[k] = next[k];
+    if (r + step < a.rows) fetch(r + step);
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+      if (lane + k * 32 < packs)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += value(raw[k], i);
+    const float mean = warp_sum(s) * inv_h;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+      if (lane + k * 32 < packs)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float c = value(raw[k], i) - mean;
+          s += c * c;
+        }
+    const float rstd = 1.f / sqrtf(warp_sum(s) * inv_h + a.eps);
+    T* y = static_cast<T*>(a.out) + r * a.H;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      if (lane + k * 32 < packs) {
+        float o[V];
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+          const float4 w = param[0][k * (V / 4) + q][lane], b = param[1][k * (V / 4) + q][lane];
+          o[4 * q] = (value(raw[k], 4 * q) - mean) * rstd * w.x + b.x;
+          o[4 * q + 1] = (value(raw[k], 4 * q + 1) - mean) * rstd * w.y + b.y;
+          o[4 * q + 2] = (value(raw[k], 4 * q + 2) - mean) * rstd * w.z + b.z;
+          o[4 * q + 3] = (value(raw[k], 4 * q + 3) - mean) * rstd * w.w + b.w;
+        }
+        store_pack<T, V>(y + (lane + k * 32) * V, o);
       }
     }
     if (lane == 0) {
@@ -182,42 +286,39 @@ __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(const NormArgs a) {
   }
 }
 
-template <typename T, int V, int VPT, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kWarpRows) ln_bwd_kernel(const NormArgs a) {
-  extern __shared__ float smem[];  // warp-a-row: the warps' column sums at the end
-  __shared__ float2 scratch[32];
-  const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31;
-  const int warp = threadIdx.x >> 5;
-  const int width = BLOCK ? blockDim.x : 32;
-  const long first = BLOCK ? blockIdx.x : blockIdx.x * static_cast<long>(kWarpRows) + warp;
-  const long step = BLOCK ? gridDim.x : gridDim.x * static_cast<long>(kWarpRows);
+// Backward of narrow rows, a warp each (packs <= 32 VPT).
+template <typename T, int V, int VPT>
+__global__ void __launch_bounds__(32 * kWarpRows) ln_bwd_warp_kernel(const NormArgs a) {
+  __shared__ float sum[kWarpRows / 2][2 * 32 * VPT * V];  // half of the warps' column sums
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int packs = a.H / V;
   const float inv_h = 1.f / static_cast<float>(a.H);
   float dw[VPT * V], db[VPT * V];
 #pragma unroll
   for (int i = 0; i < VPT * V; ++i) dw[i] = db[i] = 0.f;
-  for (long r = first; r < a.rows; r += step) {
-    const Pack<T, V>* x = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.x) + r * a.ldx);
-    const Pack<T, V>* dy = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.dy) + r * a.ldy);
+  for (long r = blockIdx.x * static_cast<long>(kWarpRows) + warp; r < a.rows;
+       r += gridDim.x * static_cast<long>(kWarpRows)) {
+    const T* x = static_cast<const T*>(a.x) + r * a.ldx;
+    const T* dy = static_cast<const T*>(a.dy) + r * a.ldy;
     Pack<T, V> rx[VPT], rd[VPT];
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
-      if (lane + k * width < packs) {
-        rx[k] = x[lane + k * width];
-        rd[k] = dy[lane + k * width];
+      if (lane + k * 32 < packs) {
+        rx[k] = load_raw<T, V>(x + (lane + k * 32) * V);
+        rd[k] = load_raw<T, V>(dy + (lane + k * 32) * V);
       }
     const float mean = a.mean[r], rstd = a.rstd[r];
     float sa = 0.f, san = 0.f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int p = lane + k * width;
+      const int p = lane + k * 32;
       if (p < packs) {
         float w[V];
         load_param<T, V>(a.w, a.w32, static_cast<long>(p) * V, w);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float g = to_f(rd[k].v[i]);
-          const float n = (to_f(rx[k].v[i]) - mean) * rstd;
+          const float g = value(rd[k], i);
+          const float n = (value(rx[k], i) - mean) * rstd;
           dw[k * V + i] += g * n;
           db[k * V + i] += g;
           sa += g * w[i];
@@ -225,29 +326,48 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kWarpRows) ln_bwd_kernel(co
         }
       }
     }
-    const float2 sums = row_sum2<BLOCK>(sa, san, scratch);
-    const float ma = sums.x * inv_h, man = sums.y * inv_h;
+    const float ma = warp_sum(sa) * inv_h, man = warp_sum(san) * inv_h;
     T* dx = static_cast<T*>(a.out) + r * a.H;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int p = lane + k * width;
+      const int p = lane + k * 32;
       if (p < packs) {
         float w[V], o[V];
         load_param<T, V>(a.w, a.w32, static_cast<long>(p) * V, w);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float n = (to_f(rx[k].v[i]) - mean) * rstd;
-          o[i] = rstd * (to_f(rd[k].v[i]) * w[i] - ma - n * man);
+          const float n = (value(rx[k], i) - mean) * rstd;
+          o[i] = rstd * (value(rd[k], i) * w[i] - ma - n * man);
         }
         store_pack<T, V>(dx + static_cast<long>(p) * V, o);
       }
     }
   }
+  // the upper half of the warps hands its sums to the lower half until one has them all;
+  // value-major, so that a warp's accesses fall into different banks
+  for (int half = kWarpRows / 2; half > 0; half >>= 1) {
+    if (warp >= half && warp < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < VPT * V; ++i) {
+        sum[warp - half][i * 32 + lane] = dw[i];
+        sum[warp - half][(VPT * V + i) * 32 + lane] = db[i];
+      }
+    }
+    __syncthreads();
+    if (warp < half) {
+#pragma unroll
+      for (int i = 0; i < VPT * V; ++i) {
+        dw[i] += sum[warp][i * 32 + lane];
+        db[i] += sum[warp][(VPT * V + i) * 32 + lane];
+      }
+    }
+    __syncthreads();
+  }
   float* part = a.part + static_cast<long>(blockIdx.x) * 2 * a.H;
-  if constexpr (BLOCK) {
+  if (warp == 0) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int p = lane + k * width;
+      const int p = lane + k * 32;
       if (p < packs)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -255,25 +375,118 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kWarpRows) ln_bwd_kernel(co
           part[a.H + p * V + i] = db[k * V + i];
         }
     }
-  } else {
-    // one warp after the other adds its sums: a fixed order
-    for (int w = 0; w < kWarpRows; ++w) {
-      if (warp == w) {
+  }
+}
+
+// Backward of wider rows: thread t owns the packs t + k blockDim.x of every row
+// of its block and takes R rows at a time; the next R are on their way meanwhile.
+template <typename T, int V, int VPT, int R>
+__global__ void __launch_bounds__(512) ln_bwd_kernel(const NormArgs a) {
+  __shared__ float part_s[2 * R][17];   // [row sum][warp]
+  __shared__ float sums[2 * R];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int packs = a.H / V;
+  const float inv_h = 1.f / static_cast<float>(a.H);
+  const long per = (a.rows + gridDim.x - 1) / gridDim.x;
+  const long begin = min(a.rows, blockIdx.x * per), end = min(a.rows, begin + per);
+  float dw[VPT * V], db[VPT * V];
+#pragma unroll
+  for (int i = 0; i < VPT * V; ++i) dw[i] = db[i] = 0.f;
+  Pack<T, V> nx[R][VPT], nd[R][VPT];
+  const auto fetch = [&](long r0) {
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (r0 + j < end) {
+        const T* x = static_cast<const T*>(a.x) + (r0 + j) * a.ldx;
+        const T* dy = static_cast<const T*>(a.dy) + (r0 + j) * a.ldy;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-          const int p = lane + k * width;
-          if (p < packs)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              float* at = smem + p * V + i;
-              at[0] = (w == 0 ? 0.f : at[0]) + dw[k * V + i];
-              at[a.H] = (w == 0 ? 0.f : at[a.H]) + db[k * V + i];
-            }
+          const int p = threadIdx.x + k * blockDim.x;
+          if (p < packs) {
+            nx[j][k] = load_raw<T, V>(x + static_cast<long>(p) * V);
+            nd[j][k] = load_raw<T, V>(dy + static_cast<long>(p) * V);
+          }
         }
       }
-      __syncthreads();
+  };
+  fetch(begin);
+  for (long r0 = begin; r0 < end; r0 += R) {
+    Pack<T, V> rx[R][VPT], rd[R][VPT];
+    float mean[R], rstd[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        rx[j][k] = nx[j][k];
+        rd[j][k] = nd[j][k];
+      }
+      mean[j] = r0 + j < end ? a.mean[r0 + j] : 0.f;
+      rstd[j] = r0 + j < end ? a.rstd[r0 + j] : 0.f;
     }
-    for (int c = threadIdx.x; c < 2 * a.H; c += blockDim.x) part[c] = smem[c];
+    if (r0 + R < end) fetch(r0 + R);
+    float s[2 * R];
+#pragma unroll
+    for (int j = 0; j < 2 * R; ++j) s[j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int p = threadIdx.x + k * blockDim.x;
+      if (p < packs) {
+        float w[V];
+        load_param<T, V>(a.w, a.w32, static_cast<long>(p) * V, w);
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+          if (r0 + j < end)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float g = value(rd[j][k], i);
+              const float n = (value(rx[j][k], i) - mean[j]) * rstd[j];
+              dw[k * V + i] += g * n;
+              db[k * V + i] += g;
+              s[j] += g * w[i];
+              s[R + j] += g * w[i] * n;
+            }
+      }
+    }
+    const float mine = warp_sum_many<2 * R>(s);
+    constexpr int kSpread = 32 / (2 * R);  // lanes that hold the same sum
+    if (lane % kSpread == 0) part_s[lane / kSpread][warp] = mine;
+    __syncthreads();
+    for (int j = warp; j < 2 * R; j += warps) {
+      const float v = warp_sum(lane < warps ? part_s[j][lane] : 0.f);
+      if (lane == 0) sums[j] = v * inv_h;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int p = threadIdx.x + k * blockDim.x;
+      if (p < packs) {
+        float w[V];
+        load_param<T, V>(a.w, a.w32, static_cast<long>(p) * V, w);
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+          if (r0 + j < end) {
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float n = (value(rx[j][k], i) - mean[j]) * rstd[j];
+              o[i] = rstd[j] * (value(rd[j][k], i) * w[i] - sums[j] - n * sums[R + j]);
+            }
+            store_pack<T, V>(static_cast<T*>(a.out) + (r0 + j) * a.H + static_cast<long>(p) * V, o);
+          }
+      }
+    }
+    // the next rows' first barrier keeps `sums` until every thread has read it
+  }
+  float* part = a.part + static_cast<long>(blockIdx.x) * 2 * a.H;
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    const int p = threadIdx.x + k * blockDim.x;
+    if (p < packs)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        part[p * V + i] = dw[k * V + i];
+        part[a.H + p * V + i] = db[k * V + i];
+      }
   }
 }
 
@@ -349,143 +562,194 @@ __global__ void __launch_bounds__(1024) ln_join_kernel(const float* __restrict__
 
 using NormKernel = void (*)(NormArgs);
 
-// The kernel for rows of H values, its threads per block and rows per block.
+// The kernel for rows of H values (null: the one for long rows), its threads per
+// block, and the rows that a block takes at least (0: as many blocks as stay resident).
 struct NormPlan {
-  NormKernel kernel;   // null: the long variant
+  NormKernel kernel;
   int threads;
   int rows;
 };
 
-template <typename T, int V, bool FWD, int VPT, bool BLOCK>
-NormKernel pick() {
-  if constexpr (FWD) return &ln_fwd_kernel<T, V, VPT, BLOCK>;
-  else return &ln_bwd_kernel<T, V, VPT, BLOCK>;
-}
+int threads_for(int packs, int per) { return (packs + 32 * per - 1) / (32 * per) * 32; }
 
-template <typename T, int V, bool FWD>
-NormPlan norm_plan(int packs) {
-  if (packs <= 32) return {pick<T, V, FWD, 1, false>(), 32 * kWarpRows, kWarpRows};
-  if (packs <= 64) return {pick<T, V, FWD, 2, false>(), 32 * kWarpRows, kWarpRows};
-  if (packs <= 96) return {pick<T, V, FWD, 3, false>(), 32 * kWarpRows, kWarpRows};
-  if (packs <= 128) return {pick<T, V, FWD, 4, false>(), 32 * kWarpRows, kWarpRows};
-  if (packs <= 160) return {pick<T, V, FWD, 5, false>(), 32 * kWarpRows, kWarpRows};
-  const auto threads = [&](int per) { return (packs + 32 * per - 1) / (32 * per) * 32; };
-  if (packs <= 1024) return {pick<T, V, FWD, 2, true>(), threads(2), 1};
-  if (packs <= 2048) return {pick<T, V, FWD, 4, true>(), threads(4), 1};
-  if (V == 1 && packs <= 4096) return {pick<T, V, FWD, 8, true>(), threads(8), 1};
+// many: rows for several rounds of the resident warps
+template <typename T, bool WIDE>
+NormPlan fwd_plan(int H, bool many) {
+  constexpr int V = kPackSize<T, WIDE>;
+  const int packs = H / V;
+  constexpr int T1 = 32 * kWarpRows;
+  if constexpr (WIDE) {
+    if (many && packs <= 160) {
+      if (packs <= 32) return {&ln_fwd_many_kernel<T, V, 1>, T1, 0};
+      if (packs <= 64) return {&ln_fwd_many_kernel<T, V, 2>, T1, 0};
+      if (packs <= 96) return {&ln_fwd_many_kernel<T, V, 3>, T1, 0};
+      if (packs <= 128) return {&ln_fwd_many_kernel<T, V, 4>, T1, 0};
+      return {&ln_fwd_many_kernel<T, V, 5>, T1, 0};
+    }
+  }
+  if (packs <= 32) return {&ln_fwd_kernel<T, V, 1, false>, T1, kWarpRows};
+  if (packs <= 64) return {&ln_fwd_kernel<T, V, 2, false>, T1, kWarpRows};
+  if constexpr (WIDE) {
+    if (packs <= 96) return {&ln_fwd_kernel<T, V, 3, false>, T1, kWarpRows};
+    if (packs <= 128) return {&ln_fwd_kernel<T, V, 4, false>, T1, kWarpRows};
+    if (packs <= 160) return {&ln_fwd_kernel<T, V, 5, false>, T1, kWarpRows};
+    if (packs <= 1024) return {&ln_fwd_kernel<T, V, 2, true>, threads_for(packs, 2), 1};
+    if (packs <= 2048) return {&ln_fwd_kernel<T, V, 4, true>, threads_for(packs, 4), 1};
+  } else {
+    if (packs <= 128) return {&ln_fwd_kernel<T, V, 4, false>, T1, kWarpRows};
+    if (packs <= 256) return {&ln_fwd_kernel<T, V, 8, false>, T1, kWarpRows};
+    if (packs <= 512) return {&ln_fwd_kernel<T, V, 16, false>, T1, kWarpRows};
+    if (packs <= 1024) return {&ln_fwd_kernel<T, V, 32, false>, T1, kWarpRows};
+    if (packs <= 8192) return {&ln_fwd_kernel<T, V, 16, true>, threads_for(packs, 16), 1};
+  }
   return {nullptr, 1024, 1};
 }
 
-template <typename T, bool FWD>
-NormPlan norm_plan_of(int H, bool wide) {
-  constexpr int W = kPackSize<T, true>;
-  return wide ? norm_plan<T, W, FWD>(H / W) : norm_plan<T, 1, FWD>(H);
+template <typename T, bool WIDE>
+NormPlan bwd_plan(int H) {
+  constexpr int V = kPackSize<T, WIDE>;
+  const int packs = H / V;
+  if (packs <= 32) return {&ln_bwd_warp_kernel<T, V, 1>, 32 * kWarpRows, kWarpRows};
+  if (packs <= 64) return {&ln_bwd_warp_kernel<T, V, 2>, 32 * kWarpRows, kWarpRows};
+  if constexpr (WIDE) {
+    // half packs up to 2048 columns: twice the threads, twice the rows in flight
+    if (sizeof(T) == 2 && H <= 2048) return {&ln_bwd_kernel<T, 4, 1, 4>, threads_for(H / 4, 1), 2};
+    if (packs <= 512) return {&ln_bwd_kernel<T, V, 1, 4>, threads_for(packs, 1), 1};
+    if (packs <= 1024) return {&ln_bwd_kernel<T, V, 2, 2>, threads_for(packs, 2), 1};
+    if (packs <= 2048) return {&ln_bwd_kernel<T, V, 4, 1>, threads_for(packs, 4), 1};
+  } else {
+    if (packs <= 1024) return {&ln_bwd_kernel<T, V, 2, 8>, threads_for(packs, 2), 2};
+    if (packs <= 4096) return {&ln_bwd_kernel<T, V, 8, 2>, threads_for(packs, 8), 1};
+    if (packs <= 8192) return {&ln_bwd_kernel<T, V, 16, 1>, threads_for(packs, 16), 1};
+  }
+  return {nullptr, 1024, 1};
 }
 
-void check_rows(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.dim() == 2 &&
-                  t.sizes() == like.sizes() && (t.stride(1) == 1 || t.size(1) == 1),
-              name, " must be [rows, H] of x's type and device with unit inner stride");
+// A ValueError in Python, as the CPU form's checks give.
+void require(bool ok, const char* what) {
+  if (!ok) throw std::invalid_argument(what);
 }
 
-void check_param(const torch::Tensor& p, const char* name, const torch::Tensor& x) {
-  TORCH_CHECK(p.device() == x.device() && p.dim() == 1 && p.size(0) == x.size(1) && p.is_contiguous() &&
-                  (p.scalar_type() == x.scalar_type() || p.scalar_type() == torch::kFloat32),
-              name, " must be a contiguous [H] of x's type or fp32");
+void check_param(const torch::Tensor& p, const torch::Tensor& x, const char* what) {
+  require(p.device() == x.device() && p.dim() == 1 && p.size(0) == x.size(-1) &&
+              (p.scalar_type() == x.scalar_type() || p.scalar_type() == torch::kFloat32), what);
 }
+
+// [rows, H] with unit inner stride
+torch::Tensor as_rows(const torch::Tensor& t) {
+  if (t.dim() == 2 && t.stride(1) == 1) return t;
+  torch::Tensor r = t.reshape({-1, t.size(-1)});
+  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+}
+
+void check_x(const torch::Tensor& x) {
+  require(x.is_cuda() && is_storage_type(x) && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < (1L << 30),
+          "x must be a bf16, fp16 or fp32 CUDA tensor with a last dimension to normalise");
+}
+
+constexpr unsigned kMaxBlocks = 1u << 30;
 
 }  // namespace
 
-void layer_norm_fwd(torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> b, torch::Tensor y,
-                    torch::Tensor mean, torch::Tensor rstd, double eps) {
-  TORCH_CHECK(is_storage_type(x), "x must be bf16, fp16 or fp32");
-  check_rows(x, "x", x);
-  check_rows(y, "y", x);
-  check_param(w, "weight", x);
-  if (b.has_value()) check_param(*b, "bias", x);
-  TORCH_CHECK(y.is_contiguous() && x.size(1) >= 1, "y must be contiguous and H at least 1");
-  TORCH_CHECK(mean.scalar_type() == torch::kFloat32 && rstd.scalar_type() == torch::kFloat32 &&
-                  mean.is_contiguous() && rstd.is_contiguous() && mean.numel() == x.size(0) &&
-                  rstd.numel() == x.size(0), "mean and rstd must be fp32 [rows]");
+// (y, mean, rstd)
+std::vector<torch::Tensor> layer_norm_fwd(torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> b,
+                                          double eps) {
+  check_x(x);
+  check_param(w, x, "weight must be [H] of x's type or fp32 on its device");
+  if (b.has_value()) check_param(*b, x, "bias must be [H] of x's type or fp32 on its device");
   const c10::cuda::CUDAGuard guard(x.device());
-  if (x.size(0) == 0) return;
+  const int64_t H = x.size(-1);
+  const torch::Tensor rows = x.numel() > 0 ? as_rows(x) : x;
+  const int64_t n = x.numel() / H;
+  torch::Tensor y = torch::empty(x.sizes(), x.options());
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  torch::Tensor mean = torch::empty({n}, f32), rstd = torch::empty({n}, f32);
+  if (n == 0) return {y, mean, rstd};
+  const torch::Tensor wc = w.contiguous(), bc = b.has_value() ? b->contiguous() : torch::Tensor();
   NormArgs a{};
-  a.x = x.data_ptr();
-  a.w = w.data_ptr();
-  a.b = b.has_value() ? b->data_ptr() : nullptr;
+  a.x = rows.data_ptr();
+  a.w = wc.data_ptr();
+  a.b = b.has_value() ? bc.data_ptr() : nullptr;
   a.out = y.data_ptr();
   a.mean = mean.data_ptr<float>();
   a.rstd = rstd.data_ptr<float>();
-  a.rows = x.size(0);
-  a.ldx = x.stride(0);
-  a.H = static_cast<int>(x.size(1));
+  a.rows = n;
+  a.ldx = rows.stride(0);
+  a.H = static_cast<int>(H);
   a.eps = static_cast<float>(eps);
   a.w32 = w.scalar_type() == torch::kFloat32;
   a.b32 = b.has_value() && b->scalar_type() == torch::kFloat32;
-  const bool wide = wide_rows(x) && wide_rows(y) && aligned16(a.w) && aligned16(a.b);
+  const bool wide = wide_rows(rows) && aligned16(a.w) && aligned16(a.b);
   auto stream = at::cuda::getCurrentCUDAStream();
   by_type(x.scalar_type(), [&](auto tag) {
     using T = decltype(tag);
-    const NormPlan p = norm_plan_of<T, true>(a.H, wide);
-    const long blocks = (a.rows + p.rows - 1) / p.rows;
-    if (p.kernel != nullptr) p.kernel<<<static_cast<unsigned>(std::min<long>(blocks, 1L << 30)), p.threads, 0, stream>>>(a);
-    else ln_fwd_long_kernel<T><<<static_cast<unsigned>(std::min<long>(blocks, 1L << 30)), 1024, 0, stream>>>(a);
+    const bool many = a.rows >= kSMs * 3 * kWarpRows * 4;
+    const NormPlan p = wide ? fwd_plan<T, true>(a.H, many) : fwd_plan<T, false>(a.H, many);
+    const long blocks = p.rows == 0 ? kSMs * 3 : (a.rows + p.rows - 1) / p.rows;
+    const unsigned grid = static_cast<unsigned>(std::min<long>(blocks, kMaxBlocks));
+    if (p.kernel != nullptr) p.kernel<<<grid, p.threads, 0, stream>>>(a);
+    else ln_fwd_long_kernel<T><<<grid, 1024, 0, stream>>>(a);
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {y, mean, rstd};
 }
 
-void layer_norm_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w, torch::Tensor mean, torch::Tensor rstd,
-                    torch::Tensor dx, torch::Tensor dw, c10::optional<torch::Tensor> db) {
-  TORCH_CHECK(is_storage_type(x), "x must be bf16, fp16 or fp32");
-  check_rows(x, "x", x);
-  check_rows(dy, "dy", x);
-  check_rows(dx, "dx", x);
-  check_param(w, "weight", x);
-  check_param(dw, "dw", x);
-  if (db.has_value()) check_param(*db, "db", x);
-  TORCH_CHECK(dx.is_contiguous() && x.size(1) >= 1, "dx must be contiguous and H at least 1");
-  TORCH_CHECK(mean.scalar_type() == torch::kFloat32 && rstd.scalar_type() == torch::kFloat32 &&
-                  mean.is_contiguous() && rstd.is_contiguous() && mean.numel() == x.size(0) &&
-                  rstd.numel() == x.size(0), "mean and rstd must be fp32 [rows]");
+// (dx, dw, db); db is fp32 or of x's type
+std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w, torch::Tensor mean,
+                                          torch::Tensor rstd, bool bias32) {
+  check_x(x);
+  check_param(w, x, "weight must be [H] of x's type or fp32 on its device");
+  require(dy.device() == x.device() && dy.scalar_type() == x.scalar_type() && dy.sizes() == x.sizes(),
+          "dy must be like x");
+  const int64_t H = x.size(-1), n = x.numel() / H;
+  for (const torch::Tensor& t : {mean, rstd})
+    require(t.device() == x.device() && t.scalar_type() == torch::kFloat32 && t.is_contiguous() && t.dim() == 1 &&
+                t.size(0) == n, "mean and rstd must hold one fp32 value per row of x");
   const c10::cuda::CUDAGuard guard(x.device());
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  torch::Tensor dx = torch::empty(x.sizes(), x.options());
+  torch::Tensor dw = torch::empty({H}, w.options()), db = torch::empty({H}, bias32 ? f32 : x.options());
+  if (n == 0) {
+    dw.zero_();
+    db.zero_();
+    return {dx, dw, db};
+  }
+  const torch::Tensor rows = as_rows(x), g = as_rows(dy), wc = w.contiguous();
   NormArgs a{};
-  a.x = x.data_ptr();
-  a.dy = dy.data_ptr();
-  a.w = w.data_ptr();
+  a.x = rows.data_ptr();
+  a.dy = g.data_ptr();
+  a.w = wc.data_ptr();
   a.out = dx.data_ptr();
   a.mean = mean.data_ptr<float>();
   a.rstd = rstd.data_ptr<float>();
-  a.rows = x.size(0);
-  a.ldx = x.stride(0);
-  a.ldy = dy.stride(0);
-  a.H = static_cast<int>(x.size(1));
+  a.rows = n;
+  a.ldx = rows.stride(0);
+  a.ldy = g.stride(0);
+  a.H = static_cast<int>(H);
   a.w32 = w.scalar_type() == torch::kFloat32;
-  const bool wide = wide_rows(x) && wide_rows(dy) && wide_rows(dx) && aligned16(a.w);
+  const bool wide = wide_rows(rows) && wide_rows(g) && aligned16(a.w);
   auto stream = at::cuda::getCurrentCUDAStream();
   by_type(x.scalar_type(), [&](auto tag) {
     using T = decltype(tag);
-    const NormPlan p = norm_plan_of<T, false>(a.H, wide);
+    const NormPlan p = wide ? bwd_plan<T, true>(a.H) : bwd_plan<T, false>(a.H);
     // as many blocks as run at once: each carries its column sums through its rows
-    const long per_sm = p.kernel == nullptr ? 1 : std::max(1, 512 / p.threads);
-    const int blocks = static_cast<int>(std::max<long>(1, std::min<long>((a.rows + p.rows - 1) / p.rows, kSMs * per_sm)));
-    torch::Tensor part = torch::empty({blocks, 2, a.H}, x.options().dtype(torch::kFloat32));
+    const long per_sm = p.kernel == nullptr ? 1 : std::max(1, 1024 / p.threads);
+    const int blocks = static_cast<int>(std::min<long>((a.rows + p.rows - 1) / p.rows, kSMs * per_sm));
+    torch::Tensor part = torch::empty({blocks, 2, H}, f32);
     a.part = part.data_ptr<float>();
     if (p.kernel != nullptr) {
-      const int smem = p.rows > 1 ? 2 * a.H * 4 : 0;
-      p.kernel<<<blocks, p.threads, smem, stream>>>(a);
+      p.kernel<<<blocks, p.threads, 0, stream>>>(a);
     } else {
-      if (a.rows > 0) {
-        ln_bwd_long_kernel<T><<<static_cast<unsigned>(std::min<long>(a.rows, kSMs * 2)), 1024, 0, stream>>>(a);
-        C10_CUDA_KERNEL_LAUNCH_CHECK();
-      }
+      ln_bwd_long_kernel<T><<<static_cast<unsigned>(std::min<long>(a.rows, kSMs * 2)), 1024, 0, stream>>>(a);
+      C10_CUDA_KERNEL_LAUNCH_CHECK();
       ln_cols_long_kernel<T><<<dim3((a.H + 255) / 256, blocks), 256, 0, stream>>>(a);
     }
     C10_CUDA_KERNEL_LAUNCH_CHECK();
-    ln_join_kernel<T><<<(2 * a.H + 31) / 32, dim3(32, 32), 0, stream>>>(
-        a.part, blocks, a.H, dw.data_ptr(), db.has_value() ? db->data_ptr() : nullptr,
-        dw.scalar_type() == torch::kFloat32, db.has_value() && db->scalar_type() == torch::kFloat32);
+    ln_join_kernel<T><<<(2 * a.H + 31) / 32, dim3(32, 32), 0, stream>>>(a.part, blocks, a.H, dw.data_ptr(),
+                                                                       db.data_ptr(), a.w32, bias32);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   });
+  return {dx, dw, db};
 }
 
 }  // namespace gb

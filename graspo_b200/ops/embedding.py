@@ -25,15 +25,21 @@ _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _NO_ID = -(1 << 63)
 
 
+def _check_padding(padding_idx: int, vocab: int) -> None:
+    if not 0 <= padding_idx < vocab:
+        raise ValueError(f"padding_idx {padding_idx} is outside the table of {vocab} rows")
+
+
+# The kernels' own checks, for tensors that do not reach them.
 def _check_ids(ids: torch.Tensor, device: torch.device, vocab: int, padding_idx: int | None) -> torch.Tensor:
     if ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"ids must be int64 or int32, not {ids.dtype}")
     if ids.device != device:
         raise ValueError("ids must be on the device of the table")
-    if padding_idx is not None and not 0 <= padding_idx < vocab:
-        raise ValueError(f"padding_idx {padding_idx} is outside the table of {vocab} rows")
-    flat = ids.reshape(-1).long().contiguous()
-    if not flat.is_cuda and bool(((flat < 0) | (flat >= vocab)).any()):
+    if padding_idx is not None:
+        _check_padding(padding_idx, vocab)
+    flat = ids.reshape(-1).long()
+    if bool(((flat < 0) | (flat >= vocab)).any()):
         raise IndexError("a token id is outside the table")
     return flat
 
@@ -44,14 +50,13 @@ def _check_table(t: torch.Tensor, name: str) -> None:
 
 
 def _lookup(ids: torch.Tensor, table: torch.Tensor, scale: float, padding_idx: int | None) -> torch.Tensor:
+    if table.is_cuda:
+        if padding_idx is not None:
+            _check_padding(padding_idx, table.shape[0])
+        return ext().embed_fwd(ids, table, scale, err_word(table.device))
     _check_table(table, "table")
     flat = _check_ids(ids, table.device, table.shape[0], padding_idx)
-    if not table.is_cuda:
-        return (table[flat].float() * scale).to(table.dtype).view(*ids.shape, -1)
-    y = torch.empty(flat.numel(), table.shape[1], device=table.device, dtype=table.dtype)
-    rows = table if table.stride(1) == 1 or table.shape[1] == 1 else table.contiguous()
-    ext().embed_fwd(flat, rows, y, float(scale), err_word(table.device))
-    return y.view(*ids.shape, table.shape[1])
+    return (table[flat].float() * scale).to(table.dtype).view(*ids.shape, -1)
 
 
 def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: float = 1.0,
@@ -61,31 +66,27 @@ def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: fl
     Without ``out`` it is a new tensor of ``dy``'s type.  With ``out`` [vocab, H]
     (contiguous, any of the three types) the touched rows are added to it in
     fp32 and rounded to its type; the others are not read."""
+    if dy.is_cuda:
+        if padding_idx is not None:
+            _check_padding(padding_idx, vocab)
+        n = ids.numel()
+        launches.add((n > 1024) + (out is None) + (n >= 128) + (n >= 4096) + 1)  # sort, merge, places, groups, rows
+        return ext().embed_bwd(dy, ids, vocab, out, scale, _NO_ID if padding_idx is None else padding_idx,
+                               err_word(dy.device))
     if dy.shape[:-1] != ids.shape or dy.dim() < 1 or dy.shape[-1] == 0:
         raise ValueError(f"dy {tuple(dy.shape)} must have one row per id {tuple(ids.shape)}")
-    if dy.dtype not in _TYPES:
-        raise ValueError(f"dy must be bf16, fp16 or fp32, not {dy.dtype}")
-    if vocab < 1:
-        raise ValueError("the table has no rows")
+    if dy.dtype not in _TYPES or vocab < 1:
+        raise ValueError(f"dy must be bf16, fp16 or fp32, not {dy.dtype}, and the table needs a row")
     H = dy.shape[-1]
     if out is not None:
         _check_table(out, "out")
         if out.shape != (vocab, H) or out.device != dy.device or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous [{vocab}, {H}] on the device of dy")
-    flat = _check_ids(ids, dy.device, vocab, padding_idx)
-    rows = dy.reshape(-1, H)
-    if not dy.is_cuda:
-        keep = torch.ones_like(flat, dtype=torch.bool) if padding_idx is None else flat != padding_idx
-        total = torch.zeros(vocab, H, dtype=torch.float32) if out is None else out.float()
-        total.index_add_(0, flat[keep], rows[keep].float() * scale)
-        return total.to(dy.dtype) if out is None else out.copy_(total)
-    if rows.stride(1) != 1 and H != 1:
-        rows = rows.contiguous()
-    grad = torch.empty(vocab, H, device=dy.device, dtype=dy.dtype) if out is None else out
-    launches.add(2 + (flat.numel() > 2048))        # sort, group sums and rows; a merge above one chunk
-    ext().embed_bwd(rows, flat, grad, float(scale), _NO_ID if padding_idx is None else int(padding_idx),
-                    out is not None, err_word(dy.device))
-    return grad
+    flat, rows = _check_ids(ids, dy.device, vocab, padding_idx), dy.reshape(-1, H)
+    keep = torch.ones_like(flat, dtype=torch.bool) if padding_idx is None else flat != padding_idx
+    total = torch.zeros(vocab, H, dtype=torch.float32) if out is None else out.float()
+    total.index_add_(0, flat[keep], rows[keep].float() * scale)
+    return total.to(dy.dtype) if out is None else out.copy_(total)
 
 
 class _Embedding(torch.autograd.Function):

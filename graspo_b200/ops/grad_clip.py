@@ -57,10 +57,8 @@ def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     if dev.type != "cuda":
         _check(grads, [])
         return _norm_torch(grads)
-    norm = torch.empty((), device=dev, dtype=torch.float32)
     launches.add(-(-len(grads) // _PER_LAUNCH))
-    ext().grad_norm(grads, norm)
-    return norm
+    return ext().grad_norm(grads, dev.index if dev.index is not None else torch.cuda.current_device())
 
 
 def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float,
@@ -84,7 +82,5 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float,
             for g, o in zip(grads, grads if out is None else out):
                 o.copy_(g.float() * coef)
         return norm
-    norm = torch.empty((), device=dev, dtype=torch.float32)
-    launches.add(2 * -(-len(grads) // _PER_LAUNCH) - 1)
-    ext().grad_clip(grads, out or [], float(max_norm), norm)
-    return norm
+    launches.add(-(-len(grads) // _PER_LAUNCH))
+    return ext().grad_clip(grads, out or [], max_norm, dev.index if dev.index is not None else torch.cuda.current_device())
