@@ -105,7 +105,7 @@ torch::Tensor embed_bwd(torch::Tensor dy, torch::Tensor ids, int64_t vocab, c10:
                         double scale, int64_t padding, torch::Tensor err);
 std::vector<torch::Tensor> layer_norm_fwd(torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> b, double eps);
 std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w, torch::Tensor mean,
-                                          torch::Tensor rstd, bool bias32);
+                                          torch::Tensor rstd, bool bias32, torch::Tensor err);
 torch::Tensor grad_norm(std::vector<torch::Tensor> grads, int64_t device);
 torch::Tensor grad_clip(std::vector<torch::Tensor> grads, std::vector<torch::Tensor> out, double max_norm,
                         int64_t device);
@@ -206,7 +206,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_fwd", &gb::layer_norm_fwd, "layer norm with its row statistics", py::arg("x"), py::arg("w"),
         py::arg("b"), py::arg("eps"));
   m.def("layer_norm_bwd", &gb::layer_norm_bwd, "gradients of layer norm for x, weight and bias", py::arg("dy"),
-        py::arg("x"), py::arg("w"), py::arg("mean"), py::arg("rstd"), py::arg("bias32"));
+        py::arg("x"), py::arg("w"), py::arg("mean"), py::arg("rstd"), py::arg("bias32"),
+        py::arg("err"));
   m.def("grad_norm", &gb::grad_norm, "global 2-norm of many tensors", py::arg("grads"),
         py::arg("device"));
   m.def("grad_clip", &gb::grad_clip, "scale many tensors to a global 2-norm of at most max_norm", py::arg("grads"),

@@ -19,12 +19,11 @@
 //    groups of 32 equal tokens, and of 32 such groups, are added first, all at
 //    once, and a run then adds those sums: at most 62 tokens, 62 groups and its
 //    large groups one after the other.
-//  * Rows: a warp takes a few table rows and a slab of columns (neighbouring warps
-//    neighbouring slabs, so that blocks write contiguous memory), with every
-//    row's first place in the list at hand: every row is written once.  When only
-//    touched rows are wanted it takes a few places of the sorted list.  Few
-//    columns per warp rather than a block per row: most rows have no or one
-//    token, and what bounds them is the chain of dependent loads.
+//  * Rows: one kernel for rows of at most one token (most of them), one for rows
+//    of several, where runs start.  A warp takes a few rows (or places of the
+//    sorted list) and a slab of columns, neighbouring warps neighbouring slabs:
+//    blocks write contiguous memory, and the chains of dependent loads that bound
+//    a row run beside one another.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -47,15 +46,16 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTableRows = 8;         // table rows per warp
 constexpr int kListRows = 4;          // sorted places per warp
-constexpr int kLookup = 8;            // packs per thread of the lookup
+template <int N>
+constexpr int kLookup = N == 1 ? 16 : 8;  // packs per thread of the lookup
 constexpr unsigned kNoId = 0xffffffffu;  // sorts last: no row takes it
 constexpr unsigned kAll = 0xffffffffu;
 
 // Packs per lane of a slab, and rows of it in flight.
 template <int N>
 constexpr int kSlab = N == 1 ? 4 : 1;
-constexpr int kFlight = 8;       // tokens of a group: 32 registers of loads
-constexpr int kRunFlight = 4;    // tokens and sums of a run, where rows share the registers
+constexpr int kFlight = 8;       // tokens: 32 registers of loads
+constexpr int kRunFlight = 4;    // sums, which are fp32 for every type
 
 // y[t] = scale * table[id]; NaN for an id outside the table.  `lanes` threads a row.
 template <typename T, bool WIDE>
@@ -73,13 +73,13 @@ __global__ void __launch_bounds__(kThreads) embed_fwd_kernel(const int64_t* __re
     if (!ok && lane == 0) atomicExch(err + 1, kErrBadToken);
     const T* src = table + (ok ? id : 0) * ldt;
     T* dst = y + t * H;
-    for (int p0 = lane; p0 < packs; p0 += kLookup * lanes) {
-      Pack<T, N> k[kLookup];
+    for (int p0 = lane; p0 < packs; p0 += kLookup<N> * lanes) {
+      Pack<T, N> k[kLookup<N>];
 #pragma unroll
-      for (int u = 0; u < kLookup; ++u)
+      for (int u = 0; u < kLookup<N>; ++u)
         if (p0 + u * lanes < packs) k[u] = load_raw<T, N>(src + static_cast<long>(p0 + u * lanes) * N);
 #pragma unroll
-      for (int u = 0; u < kLookup; ++u)
+      for (int u = 0; u < kLookup<N>; ++u)
         if (p0 + u * lanes < packs) {
           float f[N];
 #pragma unroll
@@ -312,40 +312,11 @@ __device__ __forceinline__ void store_row(const float (&acc)[S][N], float scale,
     }
 }
 
-// A row with the run [a, b) of several tokens: tokens up to the first whole
-// group, groups up to the first large one, large groups, and back.  Kept out of
-// line, so that rows of none or one token need few registers.
+// The same for a row of at most one token, token[a] where there is one.
 template <typename T, typename O, bool ADD, int N, int S>
-__device__ __noinline__ void run_row(const GradRows& g, int a, int b, int p0, int packs, O* out) {
+__device__ __forceinline__ void put_row(const GradRows& g, int a, bool some, int p0, int packs, O* out) {
   float acc[S][N] = {};
-  const bool groups = g.group != nullptr && (a + kGroup - 1) / kGroup < b / kGroup;
-  const int ga = groups ? (a + kGroup - 1) / kGroup : 0, gb = groups ? b / kGroup : 0;
-  const bool larges = groups && g.large != nullptr && (ga + kGroup - 1) / kGroup < gb / kGroup;
-  const int la = larges ? (ga + kGroup - 1) / kGroup : 0, lb = larges ? gb / kGroup : 0;
-#pragma unroll 1
-  for (int part = 0; part < 5; ++part) {
-    if (part == 0 || part == 4) {
-      const int lo = part == 0 ? a : gb * kGroup, hi = part == 0 && groups ? ga * kGroup : b;
-      add_tokens<T, kRunFlight>(acc, g, lo, hi, p0, packs);
-      if (!groups) break;
-    } else {
-      const int lo = part == 1 ? ga : part == 2 ? la : larges ? lb * kGroup : gb;
-      const int hi = part == 2 ? lb : part == 1 && larges ? la * kGroup : gb;
-      add_sums<kRunFlight>(acc, part == 2 ? g.large : g.group, g.ldg, lo, hi, p0, packs);
-    }
-  }
-  store_row<O, ADD>(acc, g.scale, out, p0, packs);
-}
-
-// A row with the run [a, b), which may be empty.  The whole warp calls it.
-template <typename T, typename O, bool ADD, int N, int S>
-__device__ __forceinline__ void put_row(const GradRows& g, int a, int b, int p0, int packs, O* out) {
-  if (b - a > 1) {
-    run_row<T, O, ADD, N, S>(g, a, b, p0, packs, out);
-    return;
-  }
-  float acc[S][N] = {};
-  if (a < b) {
+  if (some) {
     const T* src = static_cast<const T*>(g.dy) + g.token[a] * g.ld;
 #pragma unroll
     for (int s = 0; s < S; ++s)
@@ -387,9 +358,12 @@ __global__ void __launch_bounds__(kThreads, 3) embed_group_kernel(const GradRows
     if (p0 + 32 * s < packs) store_pack<float, N>(out + group * g.ldg + static_cast<long>(p0 + 32 * s) * N, acc[s]);
 }
 
-// The whole table: a warp writes kTableRows rows' slabs, zeros where no token is.
+// The whole table but for rows of several tokens: a warp writes kTableRows rows'
+// slabs, zeros where no token is.  (Rows of several tokens in the same kernel
+// made it spill, and the spills of mostly empty rows were more traffic than the
+// rows.)
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads, 4) embed_table_kernel(const __grid_constant__ GradRows g) {
+__global__ void __launch_bounds__(kThreads) embed_table_kernel(const GradRows g) {
   constexpr int N = kPackSize<T, WIDE>, S = kSlab<N>;
   const int lane = threadIdx.x & 31;
   const int packs = g.H / N;
@@ -399,36 +373,87 @@ __global__ void __launch_bounds__(kThreads, 4) embed_table_kernel(const __grid_c
   const int rows = static_cast<int>(min(static_cast<long>(kTableRows), g.V - v0));
   const int p0 = w.pack;
   const int bound = lane <= rows ? g.start[v0 + lane] : 0;
-#pragma unroll 1
   for (int r = 0; r < rows; ++r) {
     const int a = __shfl_sync(kAll, bound, r), b = __shfl_sync(kAll, bound, r + 1);
-    put_row<T, T, false, N, S>(g, a, b, p0, packs, static_cast<T*>(g.out) + (v0 + r) * g.H);
+    if (b - a < 2) put_row<T, T, false, N, S>(g, a, a < b, p0, packs, static_cast<T*>(g.out) + (v0 + r) * g.H);
   }
 }
 
-// Adds to the touched rows of an existing gradient of type O: a warp takes the
-// runs that start in its kListRows sorted places.
+// The sorted places that a warp takes: whether a run starts there, and its id.
+struct Places {
+  unsigned near;   // id of place j0 - 1 + lane
+  int j0, j1;
+};
+
+__device__ __forceinline__ Places places_of(const GradRows& g, long item) {
+  Places p;
+  p.j0 = static_cast<int>(item) * kListRows;
+  p.j1 = min(g.tokens, p.j0 + kListRows);
+  const int at = p.j0 - 1 + static_cast<int>(threadIdx.x & 31);
+  p.near = at >= 0 && at < g.tokens ? g.id[at] : kNoId;
+  return p;
+}
+
+__device__ __forceinline__ bool run_starts(const Places& p, int j, unsigned& id, bool& single) {
+  const unsigned before = __shfl_sync(kAll, p.near, j - p.j0), after = __shfl_sync(kAll, p.near, j - p.j0 + 2);
+  id = __shfl_sync(kAll, p.near, j - p.j0 + 1);
+  single = after != id;
+  return id != kNoId && (j == 0 || before != id);
+}
+
+// Adds rows of one token to an existing gradient.
 template <typename T, typename O, bool WIDE>
-__global__ void __launch_bounds__(kThreads, 4) embed_list_kernel(const __grid_constant__ GradRows g) {
+__global__ void __launch_bounds__(kThreads) embed_single_kernel(const GradRows g) {
   constexpr int N = kPackSize<T, WIDE>, S = kSlab<N>;
-  const int lane = threadIdx.x & 31;
-  const int packs = g.H / N;
   const WarpWork w = warp_work<S>(g);
   if (w.item * kListRows >= g.tokens) return;
-  const int j0 = static_cast<int>(w.item) * kListRows, p0 = w.pack;
-  // ids of the places j0 - 1 .. j0 + 30
-  const int at = j0 - 1 + lane;
-  const unsigned near = at >= 0 && at < g.tokens ? g.id[at] : kNoId;
+  const Places at = places_of(g, w.item);
+  for (int j = at.j0; j < at.j1; ++j) {
+    unsigned id;
+    bool single;
+    if (run_starts(at, j, id, single) && single)
+      put_row<T, O, true, N, S>(g, j, true, w.pack, g.H / N, static_cast<O*>(g.out) + static_cast<long>(id) * g.H);
+  }
+}
+
+// Rows of several tokens: tokens up to the first whole group, groups up to the
+// first large one, large groups, and back.  A warp takes the runs that start in
+// its kListRows sorted places.
+template <typename T, typename O, bool ADD, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 2) embed_run_kernel(const GradRows g) {
+  constexpr int N = kPackSize<T, WIDE>, S = kSlab<N>;
+  const WarpWork w = warp_work<S>(g);
+  if (w.item * kListRows >= g.tokens) return;
+  const Places at = places_of(g, w.item);
+  const int packs = g.H / N, p0 = w.pack;
 #pragma unroll 1
-  for (int j = j0; j < min(g.tokens, j0 + kListRows); ++j) {
-    const unsigned id = __shfl_sync(kAll, near, j - j0 + 1);
-    if (id == kNoId) break;
-    if (j > 0 && __shfl_sync(kAll, near, j - j0) == id) continue;
+  for (int j = at.j0; j < at.j1; ++j) {
+    unsigned id;
+    bool single;
+    if (!run_starts(at, j, id, single) || single) continue;
     // lanes from this place on that hold the id; up to the last lane: search on
-    const unsigned same = __ballot_sync(kAll, near == id && lane > j - j0);
+    const int lane = threadIdx.x & 31;
+    const unsigned same = __ballot_sync(kAll, at.near == id && lane > j - at.j0);
     int b = j + __popc(same);
     if (same >> 31) b = lower_bound_warp(g.id, b, g.tokens, id + 1);
-    put_row<T, O, true, N, S>(g, j, b, p0, packs, static_cast<O*>(g.out) + static_cast<long>(id) * g.H);
+    const bool groups = g.group != nullptr && (j + kGroup - 1) / kGroup < b / kGroup;
+    const int ga = groups ? (j + kGroup - 1) / kGroup : 0, gb = groups ? b / kGroup : 0;
+    const bool larges = groups && g.large != nullptr && (ga + kGroup - 1) / kGroup < gb / kGroup;
+    const int la = larges ? (ga + kGroup - 1) / kGroup : 0, lb = larges ? gb / kGroup : 0;
+    float acc[S][N] = {};
+#pragma unroll 1
+    for (int part = 0; part < 5; ++part) {
+      if (part == 0 || part == 4) {
+        const int lo = part == 0 ? j : gb * kGroup, hi = part == 0 && groups ? ga * kGroup : b;
+        add_tokens<T, kFlight>(acc, g, lo, hi, p0, packs);
+        if (!groups) break;
+      } else {
+        const int lo = part == 1 ? ga : part == 2 ? la : larges ? lb * kGroup : gb;
+        const int hi = part == 2 ? lb : part == 1 && larges ? la * kGroup : gb;
+        add_sums<kRunFlight>(acc, part == 2 ? g.large : g.group, g.ldg, lo, hi, p0, packs);
+      }
+    }
+    store_row<O, ADD>(acc, g.scale, static_cast<O*>(g.out) + static_cast<long>(id) * g.H, p0, packs);
   }
 }
 
@@ -469,8 +494,9 @@ torch::Tensor embed_fwd(torch::Tensor ids, torch::Tensor table, double scale, to
   by_type(table.scalar_type(), [&](auto tag) {
     using T = decltype(tag);
     const int packs = wide ? H / kPackSize<T, true> : H;
+    const int each = wide ? kLookup<kPackSize<T, true>> : kLookup<1>;
     int lanes = 32;
-    while (lanes < kThreads && lanes * kLookup < packs) lanes <<= 1;
+    while (lanes < kThreads && lanes * each < packs) lanes <<= 1;
     const unsigned blocks = static_cast<unsigned>(std::min<long>(blocks_for(tokens, kThreads / lanes), 1L << 30));
     (wide ? embed_fwd_kernel<T, true> : embed_fwd_kernel<T, false>)<<<blocks, kThreads, 0,
                                                                       at::cuda::getCurrentCUDAStream()>>>(
@@ -561,13 +587,18 @@ torch::Tensor embed_bwd(torch::Tensor dy, torch::Tensor ids, int64_t vocab, c10:
           g.large = group_sums + groups * g.ldg;
         }
       }
+      const unsigned list_blocks = blocks_for(blocks_for(tokens, kListRows) * static_cast<long>(g.slabs), kWarps);
       if (whole) {
         embed_table_kernel<T, W>
             <<<blocks_for(blocks_for(vocab, kTableRows) * static_cast<long>(g.slabs), kWarps), kThreads, 0, stream>>>(g);
+        C10_CUDA_KERNEL_LAUNCH_CHECK();
+        if (tokens > 1) embed_run_kernel<T, T, false, W><<<list_blocks, kThreads, 0, stream>>>(g);
       } else {
         by_type(out.scalar_type(), [&](auto otag) {
-          embed_list_kernel<T, decltype(otag), W>
-              <<<blocks_for(blocks_for(tokens, kListRows) * static_cast<long>(g.slabs), kWarps), kThreads, 0, stream>>>(g);
+          using O = decltype(otag);
+          embed_single_kernel<T, O, W><<<list_blocks, kThreads, 0, stream>>>(g);
+          C10_CUDA_KERNEL_LAUNCH_CHECK();
+          if (tokens > 1) embed_run_kernel<T, O, true, W><<<list_blocks, kThreads, 0, stream>>>(g);
         });
       }
       C10_CUDA_KERNEL_LAUNCH_CHECK();

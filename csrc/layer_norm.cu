@@ -15,7 +15,7 @@
 // Backward: besides a row's two sums there are two sums per column.  A thread
 // owns a few columns for all rows of its block, so that those stay in registers,
 // and takes R rows at a time: their loads are in flight together and their 2 R
-// row sums share two barriers.  (A warp a row needs 80 registers of column sums
+// row sums share a barrier.  (A warp a row needs 80 registers of column sums
 // a thread at 1152 columns and left one block of 256 threads per SM.)  Rows of
 // up to 64 packs keep the warp-a-row form.  The blocks' column sums are joined
 // by a second, small kernel in a fixed order.
@@ -36,7 +36,8 @@ namespace gb {
 
 namespace {
 
-constexpr int kWarpRows = 8;   // rows in flight per block of the warp-a-row variants
+constexpr int kWarpRows = 8;   // rows in flight per block of the warp-a-row variants,
+constexpr int kFewRows = 4;    // and of the forward where rows are few: even shares of the SMs
 constexpr int kSMs = 148;
 
 // Sum over the threads that share a row: a warp, or the block.
@@ -126,15 +127,16 @@ struct NormArgs {
   int H;
   float eps;
   bool w32, b32;
+  int* err;           // ring kernel: set when a row's copy never arrives
 };
 
 template <typename T, int V, int VPT, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kWarpRows, BLOCK ? 1 : 3) ln_fwd_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kFewRows, BLOCK ? 1 : 8) ln_fwd_kernel(const NormArgs a) {
   __shared__ float scratch[32];
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31;
   const int width = BLOCK ? blockDim.x : 32;
-  const long first = BLOCK ? blockIdx.x : blockIdx.x * static_cast<long>(kWarpRows) + (threadIdx.x >> 5);
-  const long step = BLOCK ? gridDim.x : gridDim.x * static_cast<long>(kWarpRows);
+  const long first = BLOCK ? blockIdx.x : blockIdx.x * static_cast<long>(kFewRows) + (threadIdx.x >> 5);
+  const long step = BLOCK ? gridDim.x : gridDim.x * static_cast<long>(kFewRows);
   const int packs = a.H / V;
   const float inv_h = 1.f / static_cast<float>(a.H);
   for (long r = first; r < a.rows; r += step) {
@@ -378,104 +380,149 @@ __global__ void __launch_bounds__(32 * kWarpRows) ln_bwd_warp_kernel(const NormA
   }
 }
 
+// Two fp32 values in a 64-bit register: one instruction for both.
+struct Two {
+  unsigned long long v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(Two a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
 // Backward of wider rows: thread t owns the packs t + k blockDim.x of every row
-// of its block and takes R rows at a time; the next R are on their way meanwhile.
+// of its block and takes R rows at a time; the next R are on their way while it
+// waits for their sums.  Values past the row or past the last row are zeros, so
+// that only loads and stores ask.  Bound by instructions before the arithmetic
+// went in pairs (45 a value, 148 us at 65536 x 1152).
 template <typename T, int V, int VPT, int R>
-__global__ void __launch_bounds__(512) ln_bwd_kernel(const NormArgs a) {
-  __shared__ float part_s[2 * R][17];   // [row sum][warp]
-  __shared__ float sums[2 * R];
+__global__ void __maxnreg__(V * VPT * R <= 16 ? 104 : 128) ln_bwd_kernel(const NormArgs a) {
+  constexpr int E = V * VPT;            // values per thread and row
+  static_assert(E % 2 == 0, "pairs");
+  __shared__ float part_s[2][2 * R][17];   // [turn][row sum][warp]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int packs = a.H / V;
   const float inv_h = 1.f / static_cast<float>(a.H);
   const long per = (a.rows + gridDim.x - 1) / gridDim.x;
   const long begin = min(a.rows, blockIdx.x * per), end = min(a.rows, begin + per);
-  float dw[VPT * V], db[VPT * V];
+  Two w[E / 2], dw[E / 2], db[E / 2];
+  {
+    float f[E] = {};
 #pragma unroll
-  for (int i = 0; i < VPT * V; ++i) dw[i] = db[i] = 0.f;
-  Pack<T, V> nx[R][VPT], nd[R][VPT];
-  const auto fetch = [&](long r0) {
+    for (int k = 0; k < VPT; ++k) {
+      const int p = threadIdx.x + k * blockDim.x;
+      float q[V];
+      if (p < packs) {
+        load_param<T, V>(a.w, a.w32, static_cast<long>(p) * V, q);
 #pragma unroll
-    for (int j = 0; j < R; ++j)
-      if (r0 + j < end) {
-        const T* x = static_cast<const T*>(a.x) + (r0 + j) * a.ldx;
-        const T* dy = static_cast<const T*>(a.dy) + (r0 + j) * a.ldy;
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-          const int p = threadIdx.x + k * blockDim.x;
-          if (p < packs) {
-            nx[j][k] = load_raw<T, V>(x + static_cast<long>(p) * V);
-            nd[j][k] = load_raw<T, V>(dy + static_cast<long>(p) * V);
-          }
-        }
+        for (int i = 0; i < V; ++i) f[k * V + i] = q[i];
       }
-  };
-  fetch(begin);
-  for (long r0 = begin; r0 < end; r0 += R) {
-    Pack<T, V> rx[R][VPT], rd[R][VPT];
-    float mean[R], rstd[R];
+    }
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
+    for (int i = 0; i < E / 2; ++i) {
+      w[i] = two(f[2 * i], f[2 * i + 1]);
+      dw[i] = db[i] = two(0.f, 0.f);
+    }
+  }
+  Pack<T, V> rx[R][VPT], rd[R][VPT];
+  float mean[R], rstd[R];
+  const auto fetch = [&](long r0) {
+    const T* x = static_cast<const T*>(a.x) + r0 * a.ldx + threadIdx.x * V;
+    const T* dy = static_cast<const T*>(a.dy) + r0 * a.ldy + threadIdx.x * V;
+#pragma unroll
+    for (int j = 0; j < R; ++j, x += a.ldx, dy += a.ldy) {
+      const bool row = r0 + j < end;
+      mean[j] = row ? a.mean[r0 + j] : 0.f;
+      rstd[j] = row ? a.rstd[r0 + j] : 0.f;
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
-        rx[j][k] = nx[j][k];
-        rd[j][k] = nd[j][k];
-      }
-      mean[j] = r0 + j < end ? a.mean[r0 + j] : 0.f;
-      rstd[j] = r0 + j < end ? a.rstd[r0 + j] : 0.f;
-    }
-    if (r0 + R < end) fetch(r0 + R);
-    float s[2 * R];
-#pragma unroll
-    for (int j = 0; j < 2 * R; ++j) s[j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int p = threadIdx.x + k * blockDim.x;
-      if (p < packs) {
-        float w[V];
-        load_param<T, V>(a.w, a.w32, static_cast<long>(p) * V, w);
-#pragma unroll
-        for (int j = 0; j < R; ++j)
-          if (r0 + j < end)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float g = value(rd[j][k], i);
-              const float n = (value(rx[j][k], i) - mean[j]) * rstd[j];
-              dw[k * V + i] += g * n;
-              db[k * V + i] += g;
-              s[j] += g * w[i];
-              s[R + j] += g * w[i] * n;
-            }
+        rx[j][k] = rd[j][k] = Pack<T, V>{};
+        if (row && threadIdx.x + k * blockDim.x < packs) {
+          rx[j][k] = load_raw<T, V>(x + k * blockDim.x * V);
+          rd[j][k] = load_raw<T, V>(dy + k * blockDim.x * V);
+        }
       }
     }
+  };
+  int turn = 0;
+  fetch(begin);
+  for (long r0 = begin; r0 < end; r0 += R) {
+    Two n[R][E / 2], gw[R][E / 2];   // normalised values, dy w
+    float s[2 * R], scale[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const Two shift = two(-mean[j], -mean[j]), mul = two(rstd[j], rstd[j]);
+      scale[j] = rstd[j];
+      Two sa = two(0.f, 0.f), san = two(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        const int k0 = 2 * i / V, i0 = 2 * i % V, k1 = (2 * i + 1) / V, i1 = (2 * i + 1) % V;
+        const Two g = two(value(rd[j][k0], i0), value(rd[j][k1], i1));
+        n[j][i] = mul2(add2(two(value(rx[j][k0], i0), value(rx[j][k1], i1)), shift), mul);
+        gw[j][i] = mul2(g, w[i]);
+        dw[i] = fma2(g, n[j][i], dw[i]);
+        db[i] = add2(db[i], g);
+        sa = add2(sa, gw[j][i]);
+        san = fma2(gw[j][i], n[j][i], san);
+      }
+      const float2 p = both(sa), q = both(san);
+      s[j] = p.x + p.y;
+      s[R + j] = q.x + q.y;
+    }
+    fetch(r0 + R);
     const float mine = warp_sum_many<2 * R>(s);
     constexpr int kSpread = 32 / (2 * R);  // lanes that hold the same sum
-    if (lane % kSpread == 0) part_s[lane / kSpread][warp] = mine;
+    if (lane % kSpread == 0) part_s[turn][lane / kSpread][warp] = mine;
     __syncthreads();
-    for (int j = warp; j < 2 * R; j += warps) {
-      const float v = warp_sum(lane < warps ? part_s[j][lane] : 0.f);
-      if (lane == 0) sums[j] = v * inv_h;
-    }
-    __syncthreads();
+    // every warp adds the warps' parts itself: one barrier, and the other buffer next
+    float total = 0.f;
+#pragma unroll 4
+    for (int v = 0; v < warps; ++v) total += part_s[turn][lane % (2 * R)][v];
+    total *= inv_h;
+    turn ^= 1;
+    T* dx = static_cast<T*>(a.out) + r0 * a.H + threadIdx.x * V;
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int p = threadIdx.x + k * blockDim.x;
-      if (p < packs) {
-        float w[V];
-        load_param<T, V>(a.w, a.w32, static_cast<long>(p) * V, w);
+    for (int j = 0; j < R; ++j, dx += a.H) {
+      const float ma = -__shfl_sync(0xffffffffu, total, j), man = -__shfl_sync(0xffffffffu, total, R + j);
+      const Two ma2 = two(ma, ma), man2 = two(man, man), mul = two(scale[j], scale[j]);
+      float o[E];
 #pragma unroll
-        for (int j = 0; j < R; ++j)
-          if (r0 + j < end) {
-            float o[V];
+      for (int i = 0; i < E / 2; ++i) {
+        const float2 q = both(mul2(add2(fma2(n[j][i], man2, gw[j][i]), ma2), mul));
+        o[2 * i] = q.x;
+        o[2 * i + 1] = q.y;
+      }
+      if (r0 + j < end) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float n = (value(rx[j][k], i) - mean[j]) * rstd[j];
-              o[i] = rstd[j] * (value(rd[j][k], i) * w[i] - sums[j] - n * sums[R + j]);
-            }
-            store_pack<T, V>(static_cast<T*>(a.out) + (r0 + j) * a.H + static_cast<long>(p) * V, o);
+        for (int k = 0; k < VPT; ++k)
+          if (threadIdx.x + k * blockDim.x < packs) {
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = o[k * V + i];
+            store_pack<T, V>(dx + k * blockDim.x * V, f);
           }
       }
     }
-    // the next rows' first barrier keeps `sums` until every thread has read it
   }
   float* part = a.part + static_cast<long>(blockIdx.x) * 2 * a.H;
 #pragma unroll
@@ -484,9 +531,134 @@ __global__ void __launch_bounds__(512) ln_bwd_kernel(const NormArgs a) {
     if (p < packs)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        part[p * V + i] = dw[k * V + i];
-        part[a.H + p * V + i] = db[k * V + i];
+        const float2 x = both(dw[(k * V + i) / 2]), y = both(db[(k * V + i) / 2]);
+        part[p * V + i] = (k * V + i) % 2 ? x.y : x.x;
+        part[a.H + p * V + i] = (k * V + i) % 2 ? y.y : y.x;
       }
+  }
+}
+
+// The same for many rows of up to 2048 values: rows come by bulk copies into a
+// ring of shared-memory stages (R rows of x and dy each) instead of registers.
+// The register form kept 9 warps of 104 registers on an SM, whose loads in flight
+// reached 2.9 TB/s; the ring holds some 100 KB of loads whatever the registers do.
+// A stage is read before its rows' barrier and refilled after it by one thread, so
+// it needs no second barrier.  4 values per thread and row.
+constexpr int kRing = 3;
+
+template <typename T, int R>
+__global__ void __maxnreg__(80) ln_bwd_ring_kernel(const NormArgs a) {
+  constexpr int V = 4;
+  extern __shared__ __align__(128) uint8_t ring[];   // [stage][x, dy][row][H]
+  __shared__ __align__(8) uint64_t full[kRing];
+  __shared__ float part_s[2][2 * R][17];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const bool mine_in = static_cast<int>(threadIdx.x) * V < a.H;
+  const float inv_h = 1.f / static_cast<float>(a.H);
+  const uint32_t row_bytes = a.H * sizeof(T);
+  const uint32_t stage_bytes = 2 * R * row_bytes;
+  const long per = (a.rows + gridDim.x - 1) / gridDim.x;
+  const long begin = min(a.rows, blockIdx.x * per), end = min(a.rows, begin + per);
+  const auto fill = [&](long r0, int stage) {   // one thread
+    if (r0 >= end) return;
+    const int rows = static_cast<int>(min(static_cast<long>(R), end - r0));
+    mbar_arrive_expect_tx(&full[stage], 2 * rows * row_bytes);
+    uint8_t* at = ring + stage * stage_bytes;
+    for (int j = 0; j < rows; ++j) {
+      bulk_copy_g2s(at + j * row_bytes, static_cast<const T*>(a.x) + (r0 + j) * a.ldx, row_bytes, &full[stage]);
+      bulk_copy_g2s(at + (R + j) * row_bytes, static_cast<const T*>(a.dy) + (r0 + j) * a.ldy, row_bytes, &full[stage]);
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kRing; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+    for (int s = 0; s < kRing; ++s) fill(begin + s * R, s);
+  }
+  Two w[2], dw[2], db[2];
+  {
+    float f[V] = {};
+    if (mine_in) load_param<T, V>(a.w, a.w32, static_cast<long>(threadIdx.x) * V, f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i] = two(f[2 * i], f[2 * i + 1]);
+      dw[i] = db[i] = two(0.f, 0.f);
+    }
+  }
+  float mean[R], rstd[R];
+  const auto stats = [&](long r0) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      mean[j] = r0 + j < end ? a.mean[r0 + j] : 0.f;
+      rstd[j] = r0 + j < end ? a.rstd[r0 + j] : 0.f;
+    }
+  };
+  stats(begin);
+  __syncthreads();
+  int turn = 0, stage = 0;
+  uint32_t phase = 0;
+  for (long r0 = begin; r0 < end; r0 += R) {
+    mbar_wait(&full[stage], phase, a.err, kErrTmaFullTimeout);   // late rows leave the error word set
+    Two n[R][2], gw[R][2];
+    float s[2 * R], scale[R];
+    const T* at = reinterpret_cast<const T*>(ring + stage * stage_bytes) + threadIdx.x * V;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      Pack<T, V> rx{}, rd{};
+      if (mine_in && r0 + j < end) {
+        rx = load_raw<T, V>(at + j * a.H);
+        rd = load_raw<T, V>(at + (R + j) * a.H);
+      }
+      const Two shift = two(-mean[j], -mean[j]), mul = two(rstd[j], rstd[j]);
+      scale[j] = rstd[j];
+      Two sa = two(0.f, 0.f), san = two(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Two g = two(value(rd, 2 * i), value(rd, 2 * i + 1));
+        n[j][i] = mul2(add2(two(value(rx, 2 * i), value(rx, 2 * i + 1)), shift), mul);
+        gw[j][i] = mul2(g, w[i]);
+        dw[i] = fma2(g, n[j][i], dw[i]);
+        db[i] = add2(db[i], g);
+        sa = add2(sa, gw[j][i]);
+        san = fma2(gw[j][i], n[j][i], san);
+      }
+      const float2 p = both(sa), q = both(san);
+      s[j] = p.x + p.y;
+      s[R + j] = q.x + q.y;
+    }
+    stats(r0 + R);
+    const float mine = warp_sum_many<2 * R>(s);
+    constexpr int kSpread = 32 / (2 * R);
+    if (lane % kSpread == 0) part_s[turn][lane / kSpread][warp] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) fill(r0 + kRing * R, stage);  // everyone has read this stage
+    if (++stage == kRing) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    float total = 0.f;
+#pragma unroll 4
+    for (int v = 0; v < warps; ++v) total += part_s[turn][lane % (2 * R)][v];
+    total *= inv_h;
+    turn ^= 1;
+    T* dx = static_cast<T*>(a.out) + r0 * a.H + threadIdx.x * V;
+#pragma unroll
+    for (int j = 0; j < R; ++j, dx += a.H) {
+      const float ma = -__shfl_sync(0xffffffffu, total, j), man = -__shfl_sync(0xffffffffu, total, R + j);
+      const Two ma2 = two(ma, ma), man2 = two(man, man), mul = two(scale[j], scale[j]);
+      const float2 p = both(mul2(add2(fma2(n[j][0], man2, gw[j][0]), ma2), mul));
+      const float2 q = both(mul2(add2(fma2(n[j][1], man2, gw[j][1]), ma2), mul));
+      const float o[V] = {p.x, p.y, q.x, q.y};
+      if (mine_in && r0 + j < end) store_pack<T, V>(dx, o);
+    }
+  }
+  if (mine_in) {
+    float* part = a.part + static_cast<long>(blockIdx.x) * 2 * a.H + threadIdx.x * V;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 x = both(dw[i]), y = both(db[i]);
+      part[2 * i] = x.x, part[2 * i + 1] = x.y;
+      part[a.H + 2 * i] = y.x, part[a.H + 2 * i + 1] = y.y;
+    }
   }
 }
 
@@ -587,19 +759,19 @@ NormPlan fwd_plan(int H, bool many) {
       return {&ln_fwd_many_kernel<T, V, 5>, T1, 0};
     }
   }
-  if (packs <= 32) return {&ln_fwd_kernel<T, V, 1, false>, T1, kWarpRows};
-  if (packs <= 64) return {&ln_fwd_kernel<T, V, 2, false>, T1, kWarpRows};
+  if (packs <= 32) return {&ln_fwd_kernel<T, V, 1, false>, 32 * kFewRows, kFewRows};
+  if (packs <= 64) return {&ln_fwd_kernel<T, V, 2, false>, 32 * kFewRows, kFewRows};
   if constexpr (WIDE) {
-    if (packs <= 96) return {&ln_fwd_kernel<T, V, 3, false>, T1, kWarpRows};
-    if (packs <= 128) return {&ln_fwd_kernel<T, V, 4, false>, T1, kWarpRows};
-    if (packs <= 160) return {&ln_fwd_kernel<T, V, 5, false>, T1, kWarpRows};
+    if (packs <= 96) return {&ln_fwd_kernel<T, V, 3, false>, 32 * kFewRows, kFewRows};
+    if (packs <= 128) return {&ln_fwd_kernel<T, V, 4, false>, 32 * kFewRows, kFewRows};
+    if (packs <= 160) return {&ln_fwd_kernel<T, V, 5, false>, 32 * kFewRows, kFewRows};
     if (packs <= 1024) return {&ln_fwd_kernel<T, V, 2, true>, threads_for(packs, 2), 1};
     if (packs <= 2048) return {&ln_fwd_kernel<T, V, 4, true>, threads_for(packs, 4), 1};
   } else {
-    if (packs <= 128) return {&ln_fwd_kernel<T, V, 4, false>, T1, kWarpRows};
-    if (packs <= 256) return {&ln_fwd_kernel<T, V, 8, false>, T1, kWarpRows};
-    if (packs <= 512) return {&ln_fwd_kernel<T, V, 16, false>, T1, kWarpRows};
-    if (packs <= 1024) return {&ln_fwd_kernel<T, V, 32, false>, T1, kWarpRows};
+    if (packs <= 128) return {&ln_fwd_kernel<T, V, 4, false>, 32 * kFewRows, kFewRows};
+    if (packs <= 256) return {&ln_fwd_kernel<T, V, 8, false>, 32 * kFewRows, kFewRows};
+    if (packs <= 512) return {&ln_fwd_kernel<T, V, 16, false>, 32 * kFewRows, kFewRows};
+    if (packs <= 1024) return {&ln_fwd_kernel<T, V, 32, false>, 32 * kFewRows, kFewRows};
     if (packs <= 8192) return {&ln_fwd_kernel<T, V, 16, true>, threads_for(packs, 16), 1};
   }
   return {nullptr, 1024, 1};
@@ -614,9 +786,10 @@ NormPlan bwd_plan(int H) {
   if constexpr (WIDE) {
     // half packs up to 2048 columns: twice the threads, twice the rows in flight
     if (sizeof(T) == 2 && H <= 2048) return {&ln_bwd_kernel<T, 4, 1, 4>, threads_for(H / 4, 1), 2};
-    if (packs <= 512) return {&ln_bwd_kernel<T, V, 1, 4>, threads_for(packs, 1), 1};
+    if (packs <= 512) return {&ln_bwd_kernel<T, V, 1, 16 / V>, threads_for(packs, 1), 1};
     if (packs <= 1024) return {&ln_bwd_kernel<T, V, 2, 2>, threads_for(packs, 2), 1};
-    if (packs <= 2048) return {&ln_bwd_kernel<T, V, 4, 1>, threads_for(packs, 4), 1};
+    if constexpr (sizeof(T) == 4)
+      if (packs <= 2048) return {&ln_bwd_kernel<T, V, 4, 1>, threads_for(packs, 4), 1};
   } else {
     if (packs <= 1024) return {&ln_bwd_kernel<T, V, 2, 8>, threads_for(packs, 2), 2};
     if (packs <= 4096) return {&ln_bwd_kernel<T, V, 8, 2>, threads_for(packs, 8), 1};
@@ -696,7 +869,7 @@ std::vector<torch::Tensor> layer_norm_fwd(torch::Tensor x, torch::Tensor w, c10:
 
 // (dx, dw, db); db is fp32 or of x's type
 std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w, torch::Tensor mean,
-                                          torch::Tensor rstd, bool bias32) {
+                                          torch::Tensor rstd, bool bias32, torch::Tensor err) {
   check_x(x);
   check_param(w, x, "weight must be [H] of x's type or fp32 on its device");
   require(dy.device() == x.device() && dy.scalar_type() == x.scalar_type() && dy.sizes() == x.sizes(),
@@ -725,19 +898,28 @@ std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor x, tor
   a.rows = n;
   a.ldx = rows.stride(0);
   a.ldy = g.stride(0);
+  a.err = err.data_ptr<int>();
   a.H = static_cast<int>(H);
   a.w32 = w.scalar_type() == torch::kFloat32;
   const bool wide = wide_rows(rows) && wide_rows(g) && aligned16(a.w);
   auto stream = at::cuda::getCurrentCUDAStream();
   by_type(x.scalar_type(), [&](auto tag) {
     using T = decltype(tag);
-    const NormPlan p = wide ? bwd_plan<T, true>(a.H) : bwd_plan<T, false>(a.H);
+    NormPlan p = wide ? bwd_plan<T, true>(a.H) : bwd_plan<T, false>(a.H);
+    constexpr int kRingRows = 4;
+    const int ring_bytes = kRing * 2 * kRingRows * a.H * static_cast<int>(sizeof(T));
+    // several rounds of the ring per block, rows wide enough for some warps, and two blocks' rings on an SM
+    const bool ring = wide && a.rows >= kSMs * 2 * kRingRows * 4 && a.H >= 512 && a.H <= 2048 && ring_bytes <= 100 * 1024;
+    if (ring) p = {&ln_bwd_ring_kernel<T, kRingRows>, threads_for(a.H / 4, 1), 1};
     // as many blocks as run at once: each carries its column sums through its rows
-    const long per_sm = p.kernel == nullptr ? 1 : std::max(1, 1024 / p.threads);
+    const long per_sm = p.kernel == nullptr ? 1 : std::max(1, 600 / p.threads);
     const int blocks = static_cast<int>(std::min<long>((a.rows + p.rows - 1) / p.rows, kSMs * per_sm));
     torch::Tensor part = torch::empty({blocks, 2, H}, f32);
     a.part = part.data_ptr<float>();
-    if (p.kernel != nullptr) {
+    if (ring) {
+      C10_CUDA_CHECK(cudaFuncSetAttribute(p.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_bytes));
+      p.kernel<<<blocks, p.threads, ring_bytes, stream>>>(a);
+    } else if (p.kernel != nullptr) {
       p.kernel<<<blocks, p.threads, 0, stream>>>(a);
     } else {
       ln_bwd_long_kernel<T><<<static_cast<unsigned>(std::min<long>(a.rows, kSMs * 2)), 1024, 0, stream>>>(a);

@@ -70,7 +70,7 @@ def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: fl
         if padding_idx is not None:
             _check_padding(padding_idx, vocab)
         n = ids.numel()
-        launches.add((n > 1024) + (out is None) + (n >= 128) + (n >= 4096) + 1)  # sort, merge, places, groups, rows
+        launches.add((n > 1024) + (out is None) + (n >= 128) + (n >= 4096) + 2)  # sort, merge, places, groups, rows
         return ext().embed_bwd(dy, ids, vocab, out, scale, _NO_ID if padding_idx is None else padding_idx,
                                err_word(dy.device))
     if dy.shape[:-1] != ids.shape or dy.dim() < 1 or dy.shape[-1] == 0:

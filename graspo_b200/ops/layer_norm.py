@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import torch
 
-from graspo_b200.ops._ext import ext, launches
+from graspo_b200.ops._ext import err_word, ext, launches
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -63,7 +63,8 @@ def layer_norm_backward(
         raise ValueError("the bias has x's type or fp32")
     if x.is_cuda:
         launches.add(1)                           # the join of the column sums
-        dx, dw, db = ext().layer_norm_bwd(dy, x, weight, mean, rstd, bias_dtype == torch.float32)
+        dx, dw, db = ext().layer_norm_bwd(dy, x, weight, mean, rstd, bias_dtype == torch.float32,
+                                          err_word(x.device))
         return dx, dw, db
     _check(x, weight, None)
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:

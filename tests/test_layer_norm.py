@@ -89,6 +89,27 @@ def test_many_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,H,dtype", [(4736, 512, torch.bfloat16), (4741, 1152, torch.bfloat16),
+                                          (9999, 2048, torch.float16), (4801, 1024, torch.float32),
+                                          (20001, 640, torch.float32), (15000, 1160, torch.bfloat16)])
+def test_rows_through_the_shared_memory_ring(rows, H, dtype):
+    from graspo_b200.ops._ext import check_errors
+    from graspo_b200.ops.layer_norm import layer_norm_backward, layer_norm_forward
+
+    x, w, b, dy = _case(rows, H, dtype)
+    y, mean, rstd = layer_norm_forward(x, w, b, 1e-6)
+    want, bound = _oracle(x, w, b, dy, 1e-6)
+    got = (y, *layer_norm_backward(dy, x, w, mean, rstd))
+    for name, g, v, e in zip(("y", "dx", "dw", "db"), got, want, bound):
+        _within(g, v, e, name)
+    gap = torch.zeros(rows, H + 16, device="cuda", dtype=dtype)      # rows with a gap
+    gap[:, :H] = x
+    again = layer_norm_backward(dy, gap[:, :H], w, mean, rstd)
+    assert all(torch.equal(p, q) for p, q in zip(got[1:], again))
+    check_errors()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_fp32_parameters_and_autograd(dtype):
     from graspo_b200.ops.layer_norm import layer_norm
