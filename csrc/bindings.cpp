@@ -94,12 +94,13 @@ void adamw(torch::Tensor p, torch::Tensor g, torch::Tensor m, torch::Tensor v, d
            c10::optional<torch::Tensor> loss, c10::optional<torch::Tensor> skipped);
 void transpose_bf16(torch::Tensor in, torch::Tensor out);
 std::vector<torch::Tensor> ce_forward(torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index,
-                                      int64_t reduction, c10::optional<torch::Tensor> grad, bool with_scale,
-                                      torch::Tensor err);
-void ce_scale(torch::Tensor token, torch::Tensor count, torch::Tensor grad, int64_t reduction, torch::Tensor scale);
-void ce_backward(torch::Tensor hc, torch::Tensor W, torch::Tensor place, torch::Tensor target, torch::Tensor count,
-                 torch::Tensor lse, torch::Tensor scale, c10::optional<torch::Tensor> dh,
-                 c10::optional<torch::Tensor> dW, int64_t piece, torch::Tensor err);
+                                      int64_t reduction, torch::Tensor err);
+std::vector<torch::Tensor> ce_backward(torch::Tensor hc, torch::Tensor state, torch::Tensor W, int64_t tokens,
+                                       torch::Tensor grad, int64_t reduction, bool want_h, bool want_w, int64_t piece,
+                                       torch::Tensor err);
+std::vector<torch::Tensor> ce_grads(torch::Tensor h, torch::Tensor W, torch::Tensor targets,
+                                    c10::optional<torch::Tensor> grad, int64_t ignore_index, int64_t reduction,
+                                    bool want_w, int64_t piece, torch::Tensor err);
 torch::Tensor embed_fwd(torch::Tensor ids, torch::Tensor table, double scale, torch::Tensor err);
 torch::Tensor embed_bwd(torch::Tensor dy, torch::Tensor ids, int64_t vocab, c10::optional<torch::Tensor> into,
                         double scale, int64_t padding, torch::Tensor err);
@@ -192,13 +193,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw", &gb::adamw);
   m.def("transpose_bf16", &gb::transpose_bf16);
   m.def("ce_forward", &gb::ce_forward,
-        "cross entropy over a vocabulary projection: losses and the state of the backward", py::arg("h"), py::arg("W"),
-        py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"), py::arg("grad"), py::arg("with_scale"),
-        py::arg("err"));
-  m.def("ce_scale", &gb::ce_scale, "per-token weights of the cross entropy's backward from its upstream gradient");
+        "cross entropy over a vocabulary projection: the loss and the state of its backward", py::arg("h"),
+        py::arg("W"), py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"), py::arg("err"));
   m.def("ce_backward", &gb::ce_backward, "gradients of the cross entropy, in pieces of the vocabulary", py::arg("hc"),
-        py::arg("W"), py::arg("place"), py::arg("target"), py::arg("count"), py::arg("lse"), py::arg("scale"),
-        py::arg("dh"), py::arg("dW"), py::arg("piece"), py::arg("err"));
+        py::arg("state"), py::arg("W"), py::arg("tokens"), py::arg("grad"), py::arg("reduction"), py::arg("want_h"),
+        py::arg("want_w"), py::arg("piece"), py::arg("err"));
+  m.def("ce_grads", &gb::ce_grads, "the cross entropy and its gradients in one call", py::arg("h"), py::arg("W"),
+        py::arg("targets"), py::arg("grad"), py::arg("ignore_index"), py::arg("reduction"), py::arg("want_w"),
+        py::arg("piece"), py::arg("err"));
   m.def("embed_fwd", &gb::embed_fwd, "scaled embedding lookup", py::arg("ids"), py::arg("table"), py::arg("scale"),
         py::arg("err"));
   m.def("embed_bwd", &gb::embed_bwd, "gradient of the embedding table by sorted tokens", py::arg("dy"), py::arg("ids"),

@@ -1,0 +1,422 @@
+#pragma once
+// The products of the cross entropy over a vocabulary projection
+// (cross_entropy.cu): a persistent tcgen05 GEMM, C[M, N] = A[M, K] B[N, K]^T,
+// fp32 accumulation, 128 x 256 tiles, whose extent in tokens is read on the
+// device (the number of trained tokens) and whose epilogues are the loss's.
+//
+//   kCeLse    rows tokens, columns vocabulary.  Per row and half tile of 128
+//             columns (max, sum of exp); the logit of the row's target.
+//   kCeGrad   the same product; d = r (exp(l - lse) - [v = y]) in bf16.
+//   kCeDh     rows tokens, columns hidden, K a vocabulary piece: fp32 sums of
+//             dh, K split into slices where there are few tiles.
+//   kCeDw     rows vocabulary, columns hidden, K the tokens: dW in bf16.
+//
+// One CTA per SM, 10 warps: TMA producer, MMA issuer, eight epilogue warps (two
+// per 32-lane quarter of the accumulator, 128 columns each).  Four epilogue warps
+// were not enough: at H = 1000 a tile's main loop is 8192 cycles, and the
+// exponentials of 128 x 256 logits took longer with one warp per scheduler (88 us
+// at 466 tokens x 50001).
+//
+// The tensor cores truncate the running sum at every step of 16 products, which
+// shrinks a logit by some 1e-9 of itself per product: 4e-6 at H = 4096, seen as
+// 2.5e-5 in every loss.  kCeLse therefore takes the reduction in segments of
+// kSegment K-blocks and adds those in registers, round to nearest.  The other
+// products end in bf16, where 4e-6 is nothing.
+#include "gemm_tc.cuh"
+
+namespace gb {
+
+CUtensorMap make_tmap_bf16(const void* ptr, long rows, long cols, long ld, int box_rows);  // gemm_tc.cu
+
+namespace ce {
+
+enum Mode : int { kLse, kGrad, kDh, kDw };
+
+constexpr int BN = 256;
+constexpr int kThreads = 320;
+constexpr int kEpilogue = 256;        // threads
+constexpr int kSegment = 16;          // K-blocks of 64 per fp32 partial sum of a logit
+constexpr int kLseCols = 128;         // columns per (max, sum)
+using TileCfg = Cfg<BN>;
+
+struct Args {
+  int M, N;               // rows and columns; tokens at most, where they are counted on the device
+  int kb;                 // K-blocks (kDw: at most)
+  const int* live;        // number of trained tokens
+  int* err;
+  // kLse, kGrad
+  const int64_t* target;
+  float2* part;           // [M][2 blocks]
+  float* target_logit;
+  const float* lse;
+  const float* ratio;     // r of each token
+  int n_first;            // vocabulary index of column 0
+  // results
+  void* C;
+  long ldc;
+  int kb_first;           // kDh: K-blocks of the first piece, which fix the slices
+  bool add;               // kDh: a later piece
+  const float* unit;      // kDw: what the ratios are multiples of
+};
+
+// Slices that the reduction of dh is split into: as many as fill the SMs, with at
+// least four K-blocks each and none of them empty.
+__host__ __device__ __forceinline__ int dh_slices(int live, int hidden, int kb_first, int sms) {
+  const int tiles = max(1, (live + BM - 1) / BM) * ((hidden + BN - 1) / BN);
+  const int want = max(1, min(sms / tiles, kb_first / 4));
+  const int per = (kb_first + want - 1) / want;
+  return (kb_first + per - 1) / per;
+}
+
+// Elements between the slices, whose rows are those of whole tiles.
+__host__ __device__ __forceinline__ long dh_slice_elements(int live, long ld) {
+  return static_cast<long>((live + BM - 1) / BM) * BM * ld;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 columns of a thread's TMEM lane (the 128 sums of kCeLse leave no room for 32)
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 32 bytes in one store
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 32 values of an output row; `align`: bytes that the row's chunks are multiples of.
+__device__ __forceinline__ void store_chunk(__nv_bfloat16* C, const float (&v)[32], int count, int align) {
+  if (count >= 32 && align >= 16) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
+    if (align >= 32) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t o[8] = {w[8 * q], w[8 * q + 1], w[8 * q + 2], w[8 * q + 3],
+                               w[8 * q + 4], w[8 * q + 5], w[8 * q + 6], w[8 * q + 7]};
+        store32(C + 16 * q, o);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        reinterpret_cast<uint4*>(C)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < count) C[j] = __float2bfloat16(v[j]);
+  }
+}
+
+template <int MODE, int LAYOUT>
+__global__ void __launch_bounds__(kThreads, 1)
+    ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args args) {
+  constexpr int STAGES = TileCfg::STAGES;
+  constexpr bool A_MN = (LAYOUT & 2) != 0, B_MN = (LAYOUT & 1) != 0;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_addr(smem_raw);
+  uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);  // 128-byte swizzle atoms
+  uint8_t* smA = smem;
+  uint8_t* smB = smem + STAGES * TileCfg::A_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * TileCfg::STAGE_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], kEpilogue);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, TileCfg::TMEM_COLS);
+  pdl_wait();
+  const int live = __ldcg(args.live);
+  const int M = MODE == kDw ? args.M : min(args.M, live);
+  const int kb_total = MODE == kDw ? min(args.kb, (live + BK - 1) / BK) : args.kb;
+  const int splits = MODE == kDh ? min(dh_slices(live, args.N, args.kb_first, gridDim.x), kb_total) : 1;
+  const int num_m = (M + BM - 1) / BM, num_n = (args.N + BN - 1) / BN;
+  const int units = num_m * num_n * splits;
+  constexpr int kSeg = MODE == kLse ? kSegment : 1 << 30;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Unit w = decode_unit(u, num_m, num_n, splits, kb_total);
+        for (int kb = w.kb_begin; kb < w.kb_end; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, args.err, kErrSmemEmptyTimeout)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[stage], TileCfg::STAGE_BYTES);
+          uint8_t* a_dst = smA + stage * TileCfg::A_BYTES;
+          uint8_t* b_dst = smB + stage * TileCfg::B_BYTES;
+          if constexpr (A_MN) {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j)
+              tma_load_2d(a_dst + j * kMnAtomBytes, &tmA, &full[stage], w.m_block * BM + j * 64, kb * BK);
+          } else {
+            tma_load_2d(a_dst, &tmA, &full[stage], kb * BK, w.m_block * BM);
+          }
+          if constexpr (B_MN) {
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j)
+              tma_load_2d(b_dst + j * kMnAtomBytes, &tmB, &full[stage], w.n_block * BN + j * 64, kb * BK);
+          } else {
+            tma_load_2d(b_dst, &tmB, &full[stage], kb * BK, w.n_block * BN);
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // no copy into this CTA's shared memory may be in flight at its exit
+      for (int s = 0; s < STAGES; ++s) {
+        if (!mbar_wait(&empty[stage], phase ^ 1u, args.err, kErrSmemEmptyTimeout)) break;
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_bf16(BM, BN, A_MN, B_MN);
+      constexpr uint64_t a_step = A_MN ? (2048 >> 4) : 2, b_step = B_MN ? (2048 >> 4) : 2;
+      int stage = 0, acc_iter = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Unit w = decode_unit(u, num_m, num_n, splits, kb_total);
+        for (int kb0 = w.kb_begin; kb0 < w.kb_end && ok; kb0 += kSeg) {
+          const int kb1 = w.kb_end - kb0 > kSeg ? kb0 + kSeg : w.kb_end;
+          const int acc = acc_iter & 1;
+          if (!mbar_wait(&tempty[acc], ((acc_iter >> 1) & 1) ^ 1u, args.err, kErrTmemEmptyTimeout)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait(&full[stage], phase, args.err, kErrTmaFullTimeout)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_addr = smem_addr(smA + stage * TileCfg::A_BYTES);
+            const uint32_t b_addr = smem_addr(smB + stage * TileCfg::B_BYTES);
+            const uint64_t a_desc = A_MN ? umma_desc_mn_sw128(a_addr, kMnAtomBytes, 1024) : umma_desc_k_sw128(a_addr);
+            const uint64_t b_desc = B_MN ? umma_desc_mn_sw128(b_addr, kMnAtomBytes, 1024) : umma_desc_k_sw128(b_addr);
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+              umma_bf16(tmem_base + acc * BN, a_desc + a_step * k, b_desc + b_step * k, idesc,
+                        (kb > kb0 || k > 0) ? 1u : 0u);
+            umma_commit(&empty[stage]);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          umma_commit(&tfull[acc]);
+          ++acc_iter;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp & 3;            // TMEM lanes this warp may access
+    const int half = (warp - 2) >> 2;        // which 128 columns of the tile
+    const uint32_t t_col = static_cast<uint32_t>(half * 128) + (static_cast<uint32_t>(quarter * 32) << 16);
+    const int align = (args.ldc & 15) == 0 ? 32 : (args.ldc & 7) == 0 ? 16 : 2;
+    constexpr float kLog2e = 1.4426950408889634f;
+    int acc_iter = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const Unit w = decode_unit(u, num_m, num_n, splits, kb_total);
+      const int m = w.m_block * BM + quarter * 32 + lane;
+      const int n0 = w.n_block * BN + half * 128;
+      if constexpr (MODE == kDw) {
+        if (kb_total == 0) {  // no trained token: the gradient is zero
+          const float z[32] = {};
+          for (int c = 0; c < 4; ++c)
+            if (m < M) store_chunk(static_cast<__nv_bfloat16*>(args.C) + m * args.ldc + n0 + c * 32, z,
+                                   args.N - n0 - c * 32, align);
+          continue;
+        }
+      }
+      if (w.kb_end <= w.kb_begin) continue;
+      long target = 0;
+      float lse2 = 0.f, ratio = 0.f;
+      if (m < M) {
+        if constexpr (MODE == kLse || MODE == kGrad) target = args.target[m] - args.n_first - n0;
+        if constexpr (MODE == kGrad) {
+          lse2 = args.lse[m] * kLog2e;
+          ratio = args.ratio[m];
+        }
+      }
+      if constexpr (MODE == kLse) {
+        float logit[128];
+#pragma unroll
+        for (int j = 0; j < 128; ++j) logit[j] = 0.f;
+#pragma unroll 1
+        for (int kb0 = w.kb_begin; kb0 < w.kb_end; kb0 += kSeg, ++acc_iter) {
+          const int acc = acc_iter & 1;
+          mbar_wait(&tfull[acc], (acc_iter >> 1) & 1, args.err, kErrTmemFullTimeout);
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float v[16];
+            tmem_ld16(tmem_base + acc * BN + t_col + c * 16, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) logit[c * 16 + j] += v[j];
+          }
+          tc_fence_before();
+          mbar_arrive(&tempty[acc]);
+        }
+        const int count = args.N - n0;  // columns that exist
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 128; ++j) {
+          if (j >= count) logit[j] = -INFINITY;
+          top = fmaxf(top, logit[j]);
+        }
+        // (nothing but -inf or NaN: exp(-inf) = 0 and NaN stay what they are)
+        const float base = top > -INFINITY ? top * kLog2e : 0.f;
+        float s[4] = {};
+#pragma unroll
+        for (int j = 0; j < 128; ++j) s[j & 3] += ex2(fmaf(logit[j], kLog2e, -base));
+        if (m < M) {
+          args.part[static_cast<long>(m) * (2 * num_n) + 2 * w.n_block + half] =
+              make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
+          if (target >= 0 && target < 128) {
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+              if (target == j) args.target_logit[m] = logit[j];
+          }
+        }
+      } else {
+        const int acc = acc_iter & 1;
+        const bool have = mbar_wait(&tfull[acc], (acc_iter >> 1) & 1, args.err, kErrTmemFullTimeout);
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < (have ? 4 : 0); ++c) {
+          float v[32];
+          tmem_ld32(tmem_base + acc * BN + t_col + c * 32, v);
+          const int nc = n0 + c * 32, count = args.N - nc;
+          if constexpr (MODE == kGrad) {
+            __nv_bfloat16* C = static_cast<__nv_bfloat16*>(args.C) + m * args.ldc + nc;
+            if (m < M) {
+              const int hot = static_cast<int>(target) - c * 32;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = ratio * (ex2(fmaf(v[j], kLog2e, -lse2)) - (j == hot ? 1.f : 0.f));
+              store_chunk(C, v, count, align);
+            } else if (m < (M + BK - 1) / BK * BK) {
+              // dW contracts over whole blocks of BK tokens: the rows that fill the last one are zero
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0.f;
+              store_chunk(C, v, count, align);
+            }
+          } else if constexpr (MODE == kDh) {
+            if (m < M) {
+              float* C = static_cast<float*>(args.C) + w.split * dh_slice_elements(live, args.ldc) + m * args.ldc + nc;
+              if (count >= 32) {  // ldc is a multiple of 8
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  if (args.add) {
+                    const float4 x = reinterpret_cast<const float4*>(C)[2 * q], y = reinterpret_cast<const float4*>(C)[2 * q + 1];
+                    v[8 * q] += x.x, v[8 * q + 1] += x.y, v[8 * q + 2] += x.z, v[8 * q + 3] += x.w;
+                    v[8 * q + 4] += y.x, v[8 * q + 5] += y.y, v[8 * q + 6] += y.z, v[8 * q + 7] += y.w;
+                  }
+                  uint32_t o[8];
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(v[8 * q + i]);
+                  store32(C + 8 * q, o);
+                }
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (j < count) C[j] = (args.add ? C[j] : 0.f) + v[j];
+              }
+            }
+          } else if constexpr (MODE == kDw) {
+            if (m < M) {
+              const float unit = __ldg(args.unit);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= unit;
+              store_chunk(static_cast<__nv_bfloat16*>(args.C) + m * args.ldc + nc, v, count, align);
+            }
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&tempty[acc]);
+        ++acc_iter;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TileCfg::TMEM_COLS);
+  }
+}
+
+template <int MODE, int LAYOUT>
+void launch(const CUtensorMap& a, const CUtensorMap& b, const Args& args, cudaStream_t stream, int device) {
+  auto kern = ce_gemm_kernel<MODE, LAYOUT>;
+  // MN-major operands: every address that a stage's descriptor can reach stays inside
+  constexpr int smem = TileCfg::SMEM_BYTES + (LAYOUT != 0 ? 16384 : 0);
+  static_assert(smem <= 227 * 1024, "shared memory budget");
+  static bool configured[64] = {false};
+  if (!configured[device]) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    configured[device] = true;
+  }
+  // kDh splits by the grid's size: always one CTA per SM.  The others need no more than their tiles.
+  const long tiles = static_cast<long>((args.M + BM - 1) / BM) * ((args.N + BN - 1) / BN);
+  const int grid = MODE == kDh ? num_sms(device) : static_cast<int>(std::min<long>(tiles, num_sms(device)));
+  kern<<<grid, kThreads, smem, stream>>>(a, b, args);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+}  // namespace ce
+}  // namespace gb

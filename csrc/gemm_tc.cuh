@@ -36,11 +36,6 @@
 //   kSoftmaxGrad   C = g[row] * (onehot(targets[row]) - exp(acc - lse[row]))  bf16;
 //                  the gradient of selected-token log-probs w.r.t. the logits,
 //                  produced without materialising the logits
-//   kCe*           the cross entropy over a vocabulary projection (cross_entropy.cu),
-//                  whose number of trained tokens is known to the device only
-//                  (args.live): kCeLse and kCeGrad are kLSE and kSoftmaxGrad on the
-//                  compacted tokens, kCeDh sums fp32 slices over vocabulary pieces,
-//                  kCeDw contracts over the trained tokens
 // SWAP=true stores the transpose (C[n, m]); used for small-M decode GEMMs
 // that run "swap-AB" (weights as the 128-row operand, tokens as N).
 //
@@ -56,8 +51,7 @@
 
 namespace gb {
 
-enum Epilogue : int { kStoreBF16 = 0, kSwiGLU = 1, kAtomicF32 = 2, kLSE = 3, kStoreF32 = 4, kSoftmaxGrad = 5,
-                      kCeLse = 6, kCeGrad = 7, kCeDh = 8, kCeDw = 9 };
+enum Epilogue : int { kStoreBF16 = 0, kSwiGLU = 1, kAtomicF32 = 2, kLSE = 3, kStoreF32 = 4, kSoftmaxGrad = 5 };
 
 constexpr int BM = 128;
 constexpr int BK = 64;
@@ -112,15 +106,6 @@ struct GemmArgs {
   int push_self;
   int push_rows;
   int push_fence_once;  // 1: one system fence per tile by the signalling thread (after the barrier)
-  // Cross-entropy epilogues: `live` holds the number of trained tokens n.  It is
-  // the row count of kCeLse / kCeGrad / kCeDh (M bounds it) and the length of
-  // the reduction of kCeDw.  n_first is the vocabulary index of column 0;
-  // slice the elements between the fp32 slices of kCeDh's K-splits, which are
-  // stored (add == 0) or added to (add == 1, a later vocabulary piece).
-  const int* live;
-  int n_first;
-  long slice;
-  int add;
 };
 
 template <int BN_>
@@ -341,37 +326,6 @@ __device__ __forceinline__ void swiglu_fixup_impl(const GemmArgs& args, const Un
   epi_bar();  // last_split_sw is rewritten by the next unit
 }
 
-// 32 fp32 values of an output row as bf16: four 16-byte stores, or the first
-// `count` values one by one.
-__device__ __forceinline__ void store_row_bf16(__nv_bfloat16* C, const float (&v)[32], bool wide, int count) {
-  if (wide) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint4 pk;
-      __nv_bfloat162* p2 = reinterpret_cast<__nv_bfloat162*>(&pk);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) p2[e] = __floats2bfloat162_rn(v[q * 8 + 2 * e], v[q * 8 + 2 * e + 1]);
-      *reinterpret_cast<uint4*>(C + q * 8) = pk;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < count) C[j] = __float2bfloat16(v[j]);
-  }
-}
-
-__device__ __forceinline__ void store_row_bf16_zero(const GemmArgs& args, int m, int nc) {
-  const float z[32] = {};
-  store_row_bf16(static_cast<__nv_bfloat16*>(args.C) + static_cast<long>(m) * args.ldc + nc, z,
-                 nc + 32 <= args.N && (args.ldc & 7) == 0, args.N - nc);
-}
-
-template <int BN>
-__device__ __forceinline__ void store_zero_tile(const GemmArgs& args, int m, int n0) {
-  if (m < args.M)
-    for (int c = 0; c < BN; c += 32) store_row_bf16_zero(args, m, n0 + c);
-}
-
 // LAYOUT bit 0: B (and B2) are MN-major -- given as [K, N] row-major; bit 1:
 // A (and A2) are MN-major -- given as [K, M].  MN-major tiles are loaded as
 // 64-wide column blocks of 64 K-rows (one swizzle atom column each).
@@ -400,18 +354,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  constexpr bool LIVE_M = EPI == kCeLse || EPI == kCeGrad || EPI == kCeDh;
-  constexpr bool LIVE_K = EPI == kCeDw;
-  int M = args.M, kb_main = args.kb_main;
-  if constexpr (LIVE_M || LIVE_K) {
-    pdl_wait();  // the count comes from a preceding kernel
-    const int n = __ldcg(args.live);
-    if constexpr (LIVE_M) M = min(M, n);
-    if constexpr (LIVE_K) kb_main = min(kb_main, (n + BK - 1) / BK);
-  }
-  const int num_m = (M + BM - 1) / BM;
+  const int num_m = (args.M + BM - 1) / BM;
   const int num_n = (args.N + BN - 1) / BN;
-  const int kb_total = kb_main + args.kb_ext;
+  const int kb_total = args.kb_main + args.kb_ext;
   const int units = unit_count(num_m * num_n, args.splits, args.full_tiles);
 
   if (threadIdx.x == 0) {
@@ -473,10 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int kb = w.kb_begin; kb < w.kb_end && early < STAGES; ++kb, ++early) {
             mbar_arrive_expect_tx(&full[early], C_::STAGE_BYTES);
             uint8_t* a_dst = smA + early * C_::A_BYTES;
-            if (kb < kb_main) {
+            if (kb < args.kb_main) {
               load_a(a_dst, &tmA, kb * BK, w.m_block, &full[early]);
             } else {
-              load_a(a_dst, &tmA2, (kb - kb_main) * BK, w.m_block, &full[early]);
+              load_a(a_dst, &tmA2, (kb - args.kb_main) * BK, w.m_block, &full[early]);
             }
           }
         }
@@ -490,10 +435,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* b_dst = smB + stage * C_::B_BYTES;
           if (issued < early) {
             // A half already in flight on this stage
-            if (kb < kb_main) {
+            if (kb < args.kb_main) {
               load_b(b_dst, &tmB, kb * BK, w.n_block, &full[stage]);
             } else {
-              load_b(b_dst, &tmB2, (kb - kb_main) * BK, w.n_block, &full[stage]);
+              load_b(b_dst, &tmB2, (kb - args.kb_main) * BK, w.n_block, &full[stage]);
             }
           } else {
             if (!mbar_wait(&empty[stage], phase ^ 1u, args.err, kErrSmemEmptyTimeout)) {
@@ -501,11 +446,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               break;
             }
             mbar_arrive_expect_tx(&full[stage], C_::STAGE_BYTES);
-            if (kb < kb_main) {
+            if (kb < args.kb_main) {
               load_a(a_dst, &tmA, kb * BK, w.m_block, &full[stage]);
               load_b(b_dst, &tmB, kb * BK, w.n_block, &full[stage]);
             } else {
-              const int ke = kb - kb_main;
+              const int ke = kb - args.kb_main;
               load_a(a_dst, &tmA2, ke * BK, w.m_block, &full[stage]);
               load_b(b_dst, &tmB2, ke * BK, w.n_block, &full[stage]);
             }
@@ -582,12 +527,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     int acc_iter = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const Unit w = decode_unit(u, num_m, num_n, args.splits, kb_total, args.full_tiles);
-      if constexpr (LIVE_K) {
-        if (kb_total == 0) {  // no trained token: the gradient is zero
-          store_zero_tile<BN>(args, w.m_block * BM + row_in_tile, w.n_block * BN);
-          continue;
-        }
-      }
       if (w.kb_end <= w.kb_begin) continue;
       const int acc = acc_iter & 1;
       const uint32_t acc_phase = (acc_iter >> 1) & 1;
@@ -656,15 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         } else {
-          if constexpr (EPI == kCeGrad) {
-            // The weight gradient contracts over whole blocks of BK tokens: the rows
-            // that fill the last block are zero.
-            if (m >= M) {
-              if (m < (M + BK - 1) / BK * BK) store_row_bf16_zero(args, m, nc);
-              continue;
-            }
-          }
-          if (m >= M) {
+          if (m >= args.M) {
             if constexpr (EPI == kLSE) { /* keep tcgen05.ld convergent; nothing to write */ }
             continue;
           }
@@ -798,35 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int j = 0; j < 32; ++j)
                 if (nc + j < args.N) C[j] = __float2bfloat16(v[j]);
             }
-          } else if constexpr (EPI == kCeGrad) {
-            __nv_bfloat16* C = static_cast<__nv_bfloat16*>(args.C) + static_cast<long>(m) * args.ldc + nc;
-            const float l = args.row_lse[m];
-            const float gs = args.row_scale[m];
-            const long tgt = args.targets[m] - args.n_first;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = gs * (__expf(v[j] - l) - ((nc + j) == tgt ? 1.f : 0.f));
-            store_row_bf16(C, v, full_chunk, args.N - nc);
-          } else if constexpr (EPI == kCeDh) {
-            float* C = static_cast<float*>(args.C) + w.split * args.slice + static_cast<long>(m) * args.ldc + nc;
-            if (full_chunk) {  // ldc is a multiple of 4: 16-byte accesses
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                float4 o = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                if (args.add) {
-                  const float4 p = *reinterpret_cast<const float4*>(C + q * 4);
-                  o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
-                }
-                *reinterpret_cast<float4*>(C + q * 4) = o;
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (nc + j < args.N) C[j] = (args.add ? C[j] : 0.f) + v[j];
-            }
-          } else if constexpr (EPI == kCeDw) {
-            __nv_bfloat16* C = static_cast<__nv_bfloat16*>(args.C) + static_cast<long>(m) * args.ldc + nc;
-            store_row_bf16(C, v, full_chunk && (args.ldc & 7) == 0, args.N - nc);
-          } else if constexpr (EPI == kLSE || EPI == kCeLse) {
+          } else if constexpr (EPI == kLSE) {
             float cmax = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
@@ -849,8 +752,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if constexpr ((EPI == kLSE || EPI == kCeLse) && !SWAP) {
-        if (m < M && have_acc) {
+      if constexpr (EPI == kLSE && !SWAP) {
+        if (m < args.M && have_acc) {
           float2* P = static_cast<float2*>(args.aux) + static_cast<long>(m) * args.ldaux + w.n_block;
           *P = make_float2(run_max, run_sum);
         }
@@ -919,8 +822,5 @@ GemmLauncher gemm_launcher_n128(int epi);
 GemmLauncher gemm_launcher_n64(int epi);
 GemmLauncher gemm_launcher_swap(int bn, int epi);
 GemmLauncher gemm_launcher_mn(int bn, int epi, bool swap, int layout);
-
-// Row-major bf16 matrix in boxes of [box_rows, 64] (gemm_tc.cu).
-CUtensorMap make_tmap_bf16(const void* ptr, long rows, long cols, long ld, int box_rows);
 
 }  // namespace gb

@@ -33,7 +33,8 @@ from graspo_b200.ops._ext import err_word, ext, launches
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
-def _check(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, reduction: str) -> None:
+# The kernels' own checks, for tensors that do not reach them.
+def _check(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, reduction: str, piece: int) -> None:
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(REDUCTIONS)}, not {reduction!r}")
     if weight.dim() != 2 or h.dim() < 1 or h.shape[-1] != weight.shape[1] or 0 in weight.shape:
@@ -42,10 +43,10 @@ def _check(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, reducti
         raise ValueError(f"targets {tuple(targets.shape)} must have one entry per row of h {tuple(h.shape)}")
     if targets.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"targets must be int64 or int32, not {targets.dtype}")
+    if piece < 0 or piece % 256:
+        raise ValueError("piece must be a multiple of 256")
     if h.device != weight.device or h.device != targets.device:
         raise ValueError("h, weight and targets must be on one device")
-    if h.is_cuda and not (h.dtype == weight.dtype == torch.bfloat16):
-        raise ValueError("linear_cross_entropy takes bf16 h and weight on the GPU")
 
 
 def _torch_loss(h, weight, targets, ignore_index, reduction):
@@ -61,41 +62,22 @@ def _torch_loss(h, weight, targets, ignore_index, reduction):
     return loss.sum() / max(1, loss.numel()) if reduction == "mean" else loss.sum()
 
 
-def _forward(h, weight, targets, ignore_index, reduction, grad, with_scale):
-    launches.add(3 + (reduction != "none"))       # scan, gather, products and finish are launched by one entry
-    return ext().ce_forward(h, weight, targets, ignore_index, REDUCTIONS[reduction], grad, with_scale,
-                            err_word(h.device))
-
-
-def _backward(state, weight, T, want_h, want_w, piece):
-    hc, _, place, target, count, lse, scale = state
-    dh = torch.empty(T, weight.shape[1], device=hc.device, dtype=torch.bfloat16) if want_h else None
-    dw = torch.empty(weight.shape, device=hc.device, dtype=torch.bfloat16) if want_w else None
-    launches.add(2)
-    ext().ce_backward(hc, weight, place, target, count, lse, scale, dh, dw, piece, err_word(hc.device))
-    return dh, dw
-
-
-def _rows(h, targets):
-    return h.reshape(-1, h.shape[-1]), targets.reshape(-1).long().contiguous()
-
-
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, weight, targets, ignore_index, reduction, piece):
-        rows, t = _rows(h, targets)
-        loss, *state = _forward(rows, weight, t, ignore_index, reduction, None, False)
+        launches.add(2 + (reduction != "none"))      # compaction, product, row sums (and their total)
+        loss, *state = ext().ce_forward(h, weight, targets, ignore_index, REDUCTIONS[reduction], err_word(h.device))
         ctx.save_for_backward(weight, *state)
-        ctx.shape, ctx.reduction, ctx.piece = h.shape, reduction, piece
-        return loss.view(targets.shape) if reduction == "none" else loss
+        ctx.shape, ctx.tokens, ctx.reduction, ctx.piece = h.shape, targets.numel(), reduction, piece
+        return loss
 
     @staticmethod
     def backward(ctx, g):
-        weight, *state = ctx.saved_tensors
-        T = state[2].numel()
-        scale = torch.empty_like(state[6])       # the saved state stays as it is: a second backward is possible
-        ext().ce_scale(state[1], state[4], g.float().contiguous().reshape(-1), REDUCTIONS[ctx.reduction], scale)
-        dh, dw = _backward((*state[:6], scale), weight, T, ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.piece)
+        weight, hc, state = ctx.saved_tensors
+        launches.add(4)                              # weights, three products a piece, the rows of dh
+        dh, dw = ext().ce_backward(hc, state, weight, ctx.tokens, g.float().contiguous().view(-1),
+                                   REDUCTIONS[ctx.reduction], ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+                                   ctx.piece, err_word(hc.device))
         return (None if dh is None else dh.view(ctx.shape)), dw, None, None, None, None
 
 
@@ -105,10 +87,10 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
 
     ``piece``: vocabulary columns per piece of the backward (a multiple of 256;
     0 takes as many as 256 MiB of softmax gradients hold)."""
-    _check(h, weight, targets, reduction)
-    if not h.is_cuda:
-        return _torch_loss(h, weight, targets, ignore_index, reduction)
-    return _LinearCrossEntropy.apply(h, weight, targets, int(ignore_index), reduction, int(piece))
+    if h.is_cuda and reduction in REDUCTIONS:
+        return _LinearCrossEntropy.apply(h, weight, targets, int(ignore_index), reduction, int(piece))
+    _check(h, weight, targets, reduction, piece)
+    return _torch_loss(h, weight, targets, ignore_index, reduction)
 
 
 def linear_cross_entropy_grads(
@@ -120,19 +102,20 @@ def linear_cross_entropy_grads(
     ``grad`` is the upstream gradient of the result (one value; one per token
     for ``reduction="none"``; ones when absent).  ``weight_grad=False`` leaves
     the projection's gradient out (a frozen head)."""
-    _check(h, weight, targets, reduction)
-    if grad is not None:
-        if grad.numel() != (targets.numel() if reduction == "none" else 1) or grad.device != h.device:
-            raise ValueError("grad must have one value, or one per token for reduction='none', on the device of h")
-        grad = grad.detach().reshape(-1).float().contiguous()
-    if not h.is_cuda:
-        hl, wl = h.detach().requires_grad_(True), weight.detach().requires_grad_(True)
-        with torch.enable_grad():
-            loss = _torch_loss(hl, wl, targets, ignore_index, reduction)
-            up = torch.ones_like(loss) if grad is None else grad.view(loss.shape)
-            dh, dw = torch.autograd.grad(loss, (hl, wl), up)
-        return loss.detach(), dh, dw if weight_grad else None
-    rows, t = _rows(h.detach(), targets)
-    loss, *state = _forward(rows, weight.detach(), t, int(ignore_index), reduction, grad, True)
-    dh, dw = _backward(state, weight.detach(), t.numel(), True, weight_grad, int(piece))
-    return loss.view(targets.shape) if reduction == "none" else loss, dh.view(h.shape), dw
+    if h.is_cuda and reduction in REDUCTIONS:
+        if grad is not None:
+            grad = grad.detach().float().contiguous()
+        launches.add(6 + (reduction == "none" and grad is not None))    # as the two halves, one call
+        loss, dh, dw = ext().ce_grads(h, weight, targets, grad, ignore_index, REDUCTIONS[reduction], weight_grad,
+                                      piece, err_word(h.device))
+        return loss, dh, dw
+    _check(h, weight, targets, reduction, piece)
+    if grad is not None and (grad.numel() != (targets.numel() if reduction == "none" else 1)
+                             or grad.device != h.device):
+        raise ValueError("grad must have one value, or one per token for reduction='none', on the device of h")
+    hl, wl = h.detach().requires_grad_(True), weight.detach().requires_grad_(True)
+    with torch.enable_grad():
+        loss = _torch_loss(hl, wl, targets, ignore_index, reduction)
+        up = torch.ones_like(loss) if grad is None else grad.float().view(loss.shape)
+        dh, dw = torch.autograd.grad(loss, (hl, wl), up)
+    return loss.detach(), dh, dw if weight_grad else None

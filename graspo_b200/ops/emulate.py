@@ -399,57 +399,88 @@ def sample_append_split(logits, temperature, seed, next_ids, slot, pos, kv_len, 
                   eos_id, pad_id, ignore_eos, None)
 
 
-def ce_forward(h, W, targets, ignore_index, reduction, grad, with_scale, err):
-    T, H = h.shape
-    V = W.shape[0]
-    cap, Hp = max(-(-T // 128) * 128, 128), -(-H // 8) * 8
-    live = (targets != ignore_index) & (targets >= 0) & (targets < V)
-    bad = ~live & (targets != ignore_index)
+
+def _ce_live(targets, V, ignore_index):
+    return (targets != ignore_index) & (targets >= 0) & (targets < V)
+
+
+def ce_forward(h, W, targets, ignore_index, reduction, err):
+    """The state's tensors here are the trained rows and (position, target, lse) of each."""
+    t = targets.reshape(-1).long()
+    live = _ce_live(t, W.shape[0], ignore_index)
+    bad = ~live & (t != ignore_index)
     if bool(bad.any()):
         err[1] = 8
     rows = live.nonzero()[:, 0]
-    n = rows.numel()
-    token = torch.full((cap,), -1, dtype=torch.int32)
-    token[:n] = rows.int()
-    place = torch.full((T,), -1, dtype=torch.int32)
-    place[rows] = torch.arange(n, dtype=torch.int32)
-    target = torch.zeros(cap, dtype=torch.int64)
-    target[:n] = targets[rows]
-    count = torch.tensor([n], dtype=torch.int32)
-    hc = torch.zeros(cap, Hp, dtype=h.dtype)
-    hc[:n, :H] = h[rows]
-    logits = _f(hc[:n, :H]) @ _f(W).T
-    lse = torch.zeros(cap)
-    lse[:n] = torch.logsumexp(logits, -1)
-    loss = torch.zeros(T)
+    hc = h.reshape(-1, h.shape[-1])[rows]
+    logits = _f(hc) @ _f(W).T
+    lse = torch.logsumexp(logits, -1)
+    loss = torch.zeros(t.shape)
     loss[bad] = float("nan")
-    loss[rows] = lse[:n] - logits.gather(1, target[:n, None])[:, 0]
-    scale = torch.zeros(cap)
-    if grad is not None or with_scale:
-        ce_scale(token, count, torch.ones(1) if grad is None else grad, reduction, scale)
-    if reduction:
-        loss = loss.sum() / (max(1, n) if reduction == 2 else 1)
-    return loss, hc, token, place, target, count, lse, scale
+    loss[rows] = lse - logits.gather(1, t[rows, None])[:, 0]
+    state = torch.stack([rows.double(), t[rows].double(), lse.double()])
+    if reduction == 0:
+        return loss.view(targets.shape), hc, state
+    return loss.sum() / (max(1, rows.numel()) if reduction == 2 else 1), hc, state
 
 
-def ce_scale(token, count, grad, reduction, scale):
-    n = int(count)
-    up = grad[token[:n].long()] if grad.numel() != 1 else grad.expand(n)
-    scale[:n] = up / (n if reduction == 2 else 1)
-
-
-def ce_backward(hc, W, place, target, count, lse, scale, dh, dW, piece, err):
-    n, (V, H) = int(count), W.shape
-    piece = piece or V
-    h, acc = _f(hc[:n, :H]), torch.zeros(n, H)
-    for v0 in range(0, V, piece):
-        Wv = _f(W[v0 : v0 + piece])
-        cols = torch.arange(v0, v0 + Wv.shape[0])
-        hot = (target[:n, None] == cols).float()
-        d = (scale[:n, None] * (torch.exp(h @ Wv.T - lse[:n, None]) - hot)).to(hc.dtype).float()
+def ce_backward(hc, state, W, tokens, grad, reduction, want_h, want_w, piece, err):
+    rows, target, lse = state[0].long(), state[1].long(), state[2].float()
+    n, (V, H) = rows.numel(), W.shape
+    weight = grad[rows] if reduction == 0 else grad.expand(n) / (n if reduction == 2 else 1)
+    finite = weight.abs()[torch.isfinite(weight)]
+    unit = finite.max() if finite.numel() and float(finite.max()) > 0 else torch.ones(())
+    ratio = weight / unit
+    h, acc, dw = _f(hc), torch.zeros(n, H), torch.empty(V, H, dtype=hc.dtype)
+    for v0 in range(0, V, piece or V):
+        Wv = _f(W[v0 : v0 + (piece or V)])
+        hot = (target[:, None] == torch.arange(v0, v0 + Wv.shape[0])).float()
+        d = (ratio[:, None] * (torch.exp(h @ Wv.T - lse[:, None]) - hot)).to(hc.dtype).float()
         acc += d @ Wv
-        if dW is not None:
-            dW[v0 : v0 + piece] = (d.T @ h).to(dW.dtype)
-    if dh is not None:
-        dh.zero_()
-        dh[place >= 0] = acc.to(dh.dtype)
+        dw[v0 : v0 + Wv.shape[0]] = (d.T @ h * unit).to(dw.dtype)
+    dh = torch.zeros(tokens, H, dtype=hc.dtype)
+    dh[rows] = (acc * unit).to(dh.dtype)
+    return (dh if want_h else None), (dw if want_w else None)
+
+
+def ce_grads(h, W, targets, grad, ignore_index, reduction, want_w, piece, err):
+    loss, hc, state = ce_forward(h, W, targets, ignore_index, reduction, err)
+    up = torch.ones(targets.numel() if reduction == 0 else 1) if grad is None else grad.reshape(-1)
+    dh, dw = ce_backward(hc, state, W, targets.numel(), up, reduction, True, want_w, piece, err)
+    return loss, dh.view(h.shape), dw
+
+
+def embed_fwd(ids, table, scale, err):
+    from graspo_b200.ops.embedding import embedding
+
+    return embedding(ids, table, scale=scale)
+
+
+def embed_bwd(dy, ids, vocab, into, scale, padding, err):
+    from graspo_b200.ops.embedding import embedding_grad
+
+    return embedding_grad(dy, ids, vocab, scale=scale, padding_idx=None if padding < 0 else padding, out=into)
+
+
+def layer_norm_fwd(x, w, b, eps):
+    from graspo_b200.ops.layer_norm import layer_norm_forward
+
+    return layer_norm_forward(x, w, b, eps)
+
+
+def layer_norm_bwd(dy, x, w, mean, rstd, bias32, err):
+    from graspo_b200.ops.layer_norm import layer_norm_backward
+
+    return layer_norm_backward(dy, x, w, mean, rstd, torch.float32 if bias32 else x.dtype)
+
+
+def grad_norm(grads, device):
+    from graspo_b200.ops.grad_clip import grad_norm as norm
+
+    return norm(grads)
+
+
+def grad_clip(grads, out, max_norm, device):
+    from graspo_b200.ops.grad_clip import clip_grad_norm_
+
+    return clip_grad_norm_(grads, max_norm, out=out or None)

@@ -295,6 +295,7 @@ def test_refusals():
         ((h, w, t[:3]), {}),
         ((h, w, t.float()), {}),
         ((h, w[0], t), {}),
+        ((h, w, t), {"piece": 100}),
     ]:
         with pytest.raises(ValueError):
             linear_cross_entropy(*args, **kw)
@@ -313,5 +314,5 @@ def test_refusals_on_the_gpu():
         linear_cross_entropy(h.float(), w.float(), t)
     with pytest.raises(ValueError):
         linear_cross_entropy(h, w, t.cpu())
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         linear_cross_entropy_grads(h, w, t, piece=100)
