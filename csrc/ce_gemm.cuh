@@ -36,7 +36,6 @@ constexpr int BN = 256;
 constexpr int kThreads = 320;
 constexpr int kEpilogue = 256;        // threads
 constexpr int kSegment = 16;          // K-blocks of 64 per fp32 partial sum of a logit
-constexpr int kLseCols = 128;         // columns per (max, sum)
 using TileCfg = Cfg<BN>;
 
 struct Args {
@@ -59,11 +58,14 @@ struct Args {
   const float* unit;      // kDw: what the ratios are multiples of
 };
 
-// Slices that the reduction of dh is split into: as many as fill the SMs, with at
-// least four K-blocks each and none of them empty.
+// Slices that the reduction of dh is split into, none of them empty: as many as
+// fill the SMs, with at least four K-blocks each; with more tiles than SMs two
+// where they fill the last round better (768 tiles on 148 SMs are 6 rounds, 1536
+// halves 11).
 __host__ __device__ __forceinline__ int dh_slices(int live, int hidden, int kb_first, int sms) {
   const int tiles = max(1, (live + BM - 1) / BM) * ((hidden + BN - 1) / BN);
-  const int want = max(1, min(sms / tiles, kb_first / 4));
+  int want = max(1, min(sms / tiles, kb_first / 4));
+  if (tiles >= sms && kb_first >= 64 && ((2 * tiles + sms - 1) / sms) * 100 < ((tiles + sms - 1) / sms) * 2 * 96) want = 2;
   const int per = (kb_first + want - 1) / want;
   return (kb_first + per - 1) / per;
 }
@@ -126,6 +128,28 @@ __device__ __forceinline__ void store_chunk(__nv_bfloat16* C, const float (&v)[3
 #pragma unroll
     for (int j = 0; j < 32; ++j)
       if (j < count) C[j] = __float2bfloat16(v[j]);
+  }
+}
+
+// The warp's 32 rows x 32 values, row per lane, to 32 rows of C (the lane's first
+// value at C, rows ldc apart) through 2 KB of shared memory, so that an access
+// covers 8 rows of 64 bytes instead of 32 of 16: with a row per lane the stores
+// of dW took as many cycles in L1 as 8 K-blocks of products.
+__device__ __forceinline__ void store_rows(uint8_t* stage, __nv_bfloat16* C, long ldc, const float (&v)[32], int rows) {
+  const int lane = threadIdx.x & 31;
+  uint4* s = reinterpret_cast<uint4*>(stage);
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    s[lane * 4 + (q ^ ((lane >> 1) & 3))] =
+        make_uint4(bf16_pair(v[8 * q], v[8 * q + 1]), bf16_pair(v[8 * q + 2], v[8 * q + 3]),
+                   bf16_pair(v[8 * q + 4], v[8 * q + 5]), bf16_pair(v[8 * q + 6], v[8 * q + 7]));
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2), q = lane & 3;
+    const uint4 x = s[r * 4 + (q ^ ((r >> 1) & 3))];
+    if (r < rows) reinterpret_cast<uint4*>(C + r * ldc)[q] = x;
   }
 }
 
@@ -268,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_col = static_cast<uint32_t>(half * 128) + (static_cast<uint32_t>(quarter * 32) << 16);
     const int align = (args.ldc & 15) == 0 ? 32 : (args.ldc & 7) == 0 ? 16 : 2;
     constexpr float kLog2e = 1.4426950408889634f;
+    const float unit = MODE == kDw ? __ldg(args.unit) : 1.f;
     int acc_iter = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const Unit w = decode_unit(u, num_m, num_n, splits, kb_total);
@@ -377,11 +402,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           } else if constexpr (MODE == kDw) {
-            if (m < M) {
-              const float unit = __ldg(args.unit);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= unit;
-              store_chunk(static_cast<__nv_bfloat16*>(args.C) + m * args.ldc + nc, v, count, align);
+            for (int j = 0; j < 32; ++j) v[j] *= unit;
+            __nv_bfloat16* C = static_cast<__nv_bfloat16*>(args.C) + nc;
+            if (count >= 32 && align >= 16) {
+              // the 16 KB past the stages belong to the epilogue's warps
+              store_rows(smem + STAGES * TileCfg::STAGE_BYTES + 256 + (warp - 2) * 2048, C + (m - lane) * args.ldc,
+                         args.ldc, v, M - (m - lane));
+            } else if (m < M) {
+              store_chunk(C + m * args.ldc, v, count, align);
             }
           }
         }
@@ -403,7 +432,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int MODE, int LAYOUT>
 void launch(const CUtensorMap& a, const CUtensorMap& b, const Args& args, cudaStream_t stream, int device) {
   auto kern = ce_gemm_kernel<MODE, LAYOUT>;
-  // MN-major operands: every address that a stage's descriptor can reach stays inside
+  // MN-major operands: every address that a stage's descriptor can reach stays inside,
+  // and kDw's warps stage their rows there, past the 256 bytes of barriers
   constexpr int smem = TileCfg::SMEM_BYTES + (LAYOUT != 0 ? 16384 : 0);
   static_assert(smem <= 227 * 1024, "shared memory budget");
   static bool configured[64] = {false};

@@ -37,7 +37,8 @@ namespace gb {
 
 namespace {
 
-constexpr int kRowPad = BM;     // rows of the compacted buffers come in whole GEMM tiles
+constexpr int kRowPad = BM;     // rows of the compacted buffers come in whole GEMM tiles,
+constexpr int kColumnPad = 64;  // and start on 128-byte lines
 constexpr int kBlock = 256;
 constexpr int kTokens = 32;     // tokens per block of ce_compact
 
@@ -144,10 +145,11 @@ __global__ void __launch_bounds__(kBlock) ce_compact_kernel(const int64_t* __res
 }
 
 // Rows of W with zeros in the columns [H, ldo).
+template <bool WIDE>
 __global__ void __launch_bounds__(kBlock) ce_pad_kernel(const __nv_bfloat16* __restrict__ in, long ldi, int H,
                                                           long rows, __nv_bfloat16* __restrict__ out, int ldo) {
   for (long r = blockIdx.x * (kBlock / 32L) + (threadIdx.x >> 5); r < rows; r += gridDim.x * (kBlock / 32L))
-    copy_row<false>(in + r * ldi, H, out + r * ldo, ldo);
+    copy_row<WIDE>(in + r * ldi, H, out + r * ldo, ldo);
 }
 
 // The upstream gradient of a reduced loss as every token's weight.
@@ -275,14 +277,21 @@ T* ptr(const torch::Tensor& t) {
   return reinterpret_cast<T*>(t.data_ptr());
 }
 
-// TMA reads rows of 16-byte multiples from a 16-byte boundary; W in another
-// layout is copied into one.
-torch::Tensor tma_rows(const torch::Tensor& W, cudaStream_t stream) {
+// W as TMA reads it: rows of 16-byte multiples from a 16-byte boundary.  Rows that
+// are no multiple of 32 bytes apart cross one more sector each, which every one of
+// the products that read W pays (65 against 48 us at 466 tokens x 50001 x 1000);
+// from kCopyTokens tokens on the copy costs less.
+constexpr int64_t kCopyTokens = 512;
+
+torch::Tensor tma_rows(const torch::Tensor& W, int64_t tokens, cudaStream_t stream) {
   const int64_t V = W.size(0), H = W.size(1);
-  if (W.stride(1) == 1 && W.stride(0) % 8 == 0 && W.stride(0) >= H && aligned16(W.data_ptr())) return W;
+  const bool readable = W.stride(1) == 1 && W.stride(0) % 8 == 0 && W.stride(0) >= H && aligned16(W.data_ptr());
+  if (readable && (W.stride(0) % 16 == 0 || tokens < kCopyTokens)) return W;
   const torch::Tensor src = W.stride(1) == 1 ? W : W.contiguous();
-  torch::Tensor out = torch::empty({V, round_up(H, 8)}, W.options());
-  ce_pad_kernel<<<static_cast<int>(std::min<int64_t>((V + 7) / 8, 148 * 8)), kBlock, 0, stream>>>(
+  torch::Tensor out = torch::empty({V, round_up(H, kColumnPad)}, W.options());
+  const bool wide = H % 8 == 0 && src.stride(0) % 8 == 0 && aligned16(src.data_ptr());
+  (wide ? ce_pad_kernel<true> : ce_pad_kernel<false>)<<<static_cast<int>(std::min<int64_t>((V + 7) / 8, 148 * 32)),
+                                                        kBlock, 0, stream>>>(
       ptr<__nv_bfloat16>(src), src.stride(0), static_cast<int>(H), V, ptr<__nv_bfloat16>(out),
       static_cast<int>(out.size(1)));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -306,7 +315,7 @@ Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Ten
   Forward f;
   const int device = h.get_device();
   f.T = targets.numel(), f.H = W.size(1), f.V = W.size(0);
-  f.cap = capacity(f.T), f.Hp = round_up(f.H, 8);
+  f.cap = capacity(f.T), f.Hp = round_up(f.H, kColumnPad);
   const int num_n = static_cast<int>((f.V + ce::BN - 1) / ce::BN);
   const auto f32 = h.options().dtype(torch::kFloat32);
   f.loss = torch::empty({f.T}, f32);
@@ -322,7 +331,7 @@ Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Ten
       targets.data_ptr<int64_t>(), f.T, f.V, ignore_index, ptr<__nv_bfloat16>(rows), rows.stride(0),
       static_cast<int>(f.H), st, f.loss.data_ptr<float>(), ptr<__nv_bfloat16>(f.hc), static_cast<int>(f.Hp), err);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  f.W = tma_rows(W, stream);
+  f.W = tma_rows(W, f.T, stream);
   ce::Args args{};
   args.M = static_cast<int>(f.cap);
   args.N = static_cast<int>(f.V);
@@ -356,7 +365,7 @@ void backward(const torch::Tensor& hc, const State& st, const torch::Tensor& W, 
   const int kb_first = static_cast<int>((std::min(piece, V) + BK - 1) / BK);
   torch::Tensor acc;  // room for the slices of any number of trained tokens (dh_slices)
   if (dh != nullptr)
-    acc = torch::empty({std::max<int64_t>(sms / num_n, cap / BM) * BM * Hp}, hc.options().dtype(torch::kFloat32));
+    acc = torch::empty({std::max<int64_t>(sms / num_n, 2 * cap / BM) * BM * Hp}, hc.options().dtype(torch::kFloat32));
   const CUtensorMap map_h = make_tmap_bf16(hc.data_ptr(), cap, Hp, Hp, BM);
   const CUtensorMap map_h_mn = make_tmap_bf16(hc.data_ptr(), cap, Hp, Hp, 64);
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
@@ -459,7 +468,7 @@ std::vector<torch::Tensor> ce_backward(torch::Tensor hc, torch::Tensor state, to
                                        torch::Tensor grad, int64_t reduction, bool want_h, bool want_w, int64_t piece,
                                        torch::Tensor err) {
   const int64_t H = W.size(1), V = W.size(0), cap = capacity(tokens);
-  require(hc.is_cuda() && hc.size(0) == cap && hc.size(1) == round_up(H, 8) && state.numel() == State::words(cap),
+  require(hc.is_cuda() && hc.size(0) == cap && hc.size(1) == round_up(H, kColumnPad) && state.numel() == State::words(cap),
           "state of another call");
   check_piece(piece);
   const float* g = check_grad(grad, hc, reduction, tokens);
@@ -472,7 +481,7 @@ std::vector<torch::Tensor> ce_backward(torch::Tensor hc, torch::Tensor state, to
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (want_h) dh = torch::empty({tokens, H}, hc.options());
   if (want_w) dW = torch::empty({V, H}, hc.options());
-  backward(hc, st, tma_rows(W, stream), tokens, V, H, piece, want_h ? &dh : nullptr, want_w ? &dW : nullptr,
+  backward(hc, st, tma_rows(W, tokens, stream), tokens, V, H, piece, want_h ? &dh : nullptr, want_w ? &dW : nullptr,
            torch::Tensor(), false, nullptr, err.data_ptr<int>(), stream);
   return {dh, dW};
 }

@@ -45,7 +45,7 @@ constexpr int kLargeFrom = 4096;      // ... and large groups theirs
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTableRows = 8;         // table rows per warp
-constexpr int kListRows = 4;          // sorted places per warp
+constexpr int kListRows = 28;         // sorted places per warp at most: a lane each, and one on either side
 template <int N>
 constexpr int kLookup = N == 1 ? 16 : 8;  // packs per thread of the lookup
 constexpr unsigned kNoId = 0xffffffffu;  // sorts last: no row takes it
@@ -55,7 +55,7 @@ constexpr unsigned kAll = 0xffffffffu;
 template <int N>
 constexpr int kSlab = N == 1 ? 4 : 1;
 constexpr int kFlight = 8;       // tokens: 32 registers of loads
-constexpr int kRunFlight = 4;    // sums, which are fp32 for every type
+constexpr int kSumFlight = 4;    // sums of groups, which are fp32 for every type
 
 // y[t] = scale * table[id]; NaN for an id outside the table.  `lanes` threads a row.
 template <typename T, bool WIDE>
@@ -238,6 +238,7 @@ struct GradRows {
   long ldg;
   int tokens, V, H;
   unsigned slabs;      // of columns
+  int places;          // sorted places per warp
   float scale;
   void* out;
 };
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 3) embed_group_kernel(const GradRows
   if (id == kNoId || id != g.id[lo + (LARGE ? kGroup * kGroup : kGroup) - 1]) return;
   const int packs = g.H / N;
   float acc[S][N] = {};
-  if constexpr (LARGE) add_sums<kRunFlight>(acc, g.group, g.ldg, group * kGroup, (group + 1) * kGroup, p0, packs);
+  if constexpr (LARGE) add_sums<kSumFlight>(acc, g.group, g.ldg, group * kGroup, (group + 1) * kGroup, p0, packs);
   else add_tokens<T, kFlight>(acc, g, lo, lo + kGroup, p0, packs);
 #pragma unroll
   for (int s = 0; s < S; ++s)
@@ -379,26 +380,25 @@ __global__ void __launch_bounds__(kThreads) embed_table_kernel(const GradRows g)
   }
 }
 
-// The sorted places that a warp takes: whether a run starts there, and its id.
+// The sorted places that a warp takes: bit l of `starts` where a run starts at
+// place j0 - 1 + l, of one token (`single`) or of several.
 struct Places {
   unsigned near;   // id of place j0 - 1 + lane
-  int j0, j1;
+  int j0;
+  unsigned single, several;
 };
 
 __device__ __forceinline__ Places places_of(const GradRows& g, long item) {
   Places p;
-  p.j0 = static_cast<int>(item) * kListRows;
-  p.j1 = min(g.tokens, p.j0 + kListRows);
-  const int at = p.j0 - 1 + static_cast<int>(threadIdx.x & 31);
+  const int lane = threadIdx.x & 31;
+  p.j0 = static_cast<int>(item) * g.places;
+  const int at = p.j0 - 1 + lane;
   p.near = at >= 0 && at < g.tokens ? g.id[at] : kNoId;
+  const unsigned before = __shfl_up_sync(kAll, p.near, 1), after = __shfl_down_sync(kAll, p.near, 1);
+  const bool start = lane >= 1 && lane <= g.places && p.near != kNoId && (at == 0 || before != p.near);
+  p.single = __ballot_sync(kAll, start && after != p.near);
+  p.several = __ballot_sync(kAll, start && after == p.near);
   return p;
-}
-
-__device__ __forceinline__ bool run_starts(const Places& p, int j, unsigned& id, bool& single) {
-  const unsigned before = __shfl_sync(kAll, p.near, j - p.j0), after = __shfl_sync(kAll, p.near, j - p.j0 + 2);
-  id = __shfl_sync(kAll, p.near, j - p.j0 + 1);
-  single = after != id;
-  return id != kNoId && (j == 0 || before != id);
 }
 
 // Adds rows of one token to an existing gradient.
@@ -406,34 +406,35 @@ template <typename T, typename O, bool WIDE>
 __global__ void __launch_bounds__(kThreads) embed_single_kernel(const GradRows g) {
   constexpr int N = kPackSize<T, WIDE>, S = kSlab<N>;
   const WarpWork w = warp_work<S>(g);
-  if (w.item * kListRows >= g.tokens) return;
+  if (w.item * g.places >= g.tokens) return;
   const Places at = places_of(g, w.item);
-  for (int j = at.j0; j < at.j1; ++j) {
-    unsigned id;
-    bool single;
-    if (run_starts(at, j, id, single) && single)
-      put_row<T, O, true, N, S>(g, j, true, w.pack, g.H / N, static_cast<O*>(g.out) + static_cast<long>(id) * g.H);
+  for (unsigned todo = at.single; todo != 0; todo &= todo - 1) {
+    const int l = __ffs(todo) - 1;
+    const unsigned id = __shfl_sync(kAll, at.near, l);
+    put_row<T, O, true, N, S>(g, at.j0 - 1 + l, true, w.pack, g.H / N,
+                              static_cast<O*>(g.out) + static_cast<long>(id) * g.H);
   }
 }
 
 // Rows of several tokens: tokens up to the first whole group, groups up to the
 // first large one, large groups, and back.  A warp takes the runs that start in
-// its kListRows sorted places.
+// its sorted places, the last places first: a padding token is mostly one of the
+// last ids, and its run, the longest chain, must not be the last work.
 template <typename T, typename O, bool ADD, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 2) embed_run_kernel(const GradRows g) {
   constexpr int N = kPackSize<T, WIDE>, S = kSlab<N>;
   const WarpWork w = warp_work<S>(g);
-  if (w.item * kListRows >= g.tokens) return;
-  const Places at = places_of(g, w.item);
+  const int items = (g.tokens + g.places - 1) / g.places;
+  if (w.item >= items) return;
+  const Places at = places_of(g, items - 1 - w.item);
   const int packs = g.H / N, p0 = w.pack;
 #pragma unroll 1
-  for (int j = at.j0; j < at.j1; ++j) {
-    unsigned id;
-    bool single;
-    if (!run_starts(at, j, id, single) || single) continue;
+  for (unsigned todo = at.several; todo != 0; todo &= todo - 1) {
+    const int l = __ffs(todo) - 1, j = at.j0 - 1 + l;
+    const unsigned id = __shfl_sync(kAll, at.near, l);
     // lanes from this place on that hold the id; up to the last lane: search on
     const int lane = threadIdx.x & 31;
-    const unsigned same = __ballot_sync(kAll, at.near == id && lane > j - at.j0);
+    const unsigned same = __ballot_sync(kAll, at.near == id && lane >= l);
     int b = j + __popc(same);
     if (same >> 31) b = lower_bound_warp(g.id, b, g.tokens, id + 1);
     const bool groups = g.group != nullptr && (j + kGroup - 1) / kGroup < b / kGroup;
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 2) embed_run_kernel(const GradRows g
       } else {
         const int lo = part == 1 ? ga : part == 2 ? la : larges ? lb * kGroup : gb;
         const int hi = part == 2 ? lb : part == 1 && larges ? la * kGroup : gb;
-        add_sums<kRunFlight>(acc, part == 2 ? g.large : g.group, g.ldg, lo, hi, p0, packs);
+        add_sums<kSumFlight>(acc, part == 2 ? g.large : g.group, g.ldg, lo, hi, p0, packs);
       }
     }
     store_row<O, ADD>(acc, g.scale, static_cast<O*>(g.out) + static_cast<long>(id) * g.H, p0, packs);
@@ -587,7 +588,9 @@ torch::Tensor embed_bwd(torch::Tensor dy, torch::Tensor ids, int64_t vocab, c10:
           g.large = group_sums + groups * g.ldg;
         }
       }
-      const unsigned list_blocks = blocks_for(blocks_for(tokens, kListRows) * static_cast<long>(g.slabs), kWarps);
+      // few places per warp while that fills the GPU, more where starting warps would be the work
+      g.places = static_cast<int>(std::clamp<long>(tokens * g.slabs / (148 * 64), 4, kListRows));
+      const unsigned list_blocks = blocks_for(blocks_for(tokens, g.places) * static_cast<long>(g.slabs), kWarps);
       if (whole) {
         embed_table_kernel<T, W>
             <<<blocks_for(blocks_for(vocab, kTableRows) * static_cast<long>(g.slabs), kWarps), kThreads, 0, stream>>>(g);
