@@ -47,7 +47,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kTableRows = 8;         // table rows per warp
 constexpr int kListRows = 28;         // sorted places per warp at most: a lane each, and one on either side
 template <int N>
-constexpr int kLookup = N == 1 ? 16 : 8;  // packs per thread of the lookup
+constexpr int kLookup = N == 1 ? 16 : 8;  // packs per thread of the lookup,
+constexpr int kLookupBlocks = 4;          // whose blocks stay on their SM
 constexpr unsigned kNoId = 0xffffffffu;  // sorts last: no row takes it
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -59,16 +60,19 @@ constexpr int kSumFlight = 4;    // sums of groups, which are fp32 for every typ
 
 // y[t] = scale * table[id]; NaN for an id outside the table.  `lanes` threads a row.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) embed_fwd_kernel(const int64_t* __restrict__ ids, long tokens, long V,
+__global__ void __launch_bounds__(kThreads, kLookupBlocks) embed_fwd_kernel(const int64_t* __restrict__ ids, long tokens, long V,
                                                              const T* __restrict__ table, long ldt, int H, float scale,
                                                              T* __restrict__ y, int lanes, int* __restrict__ err) {
   constexpr int N = kPackSize<T, WIDE>;
   const int per_block = kThreads / lanes;
   const int lane = threadIdx.x % lanes;
   const int packs = H / N;
-  for (long t = blockIdx.x * static_cast<long>(per_block) + threadIdx.x / lanes; t < tokens;
-       t += gridDim.x * static_cast<long>(per_block)) {
-    const long id = ids[t];
+  const long step = gridDim.x * static_cast<long>(per_block);
+  long t = blockIdx.x * static_cast<long>(per_block) + threadIdx.x / lanes;
+  long next = t < tokens ? ids[t] : 0;   // a row's id is there before its turn
+  for (; t < tokens; t += step) {
+    const long id = next;
+    if (t + step < tokens) next = ids[t + step];
     const bool ok = id >= 0 && id < V;
     if (!ok && lane == 0) atomicExch(err + 1, kErrBadToken);
     const T* src = table + (ok ? id : 0) * ldt;
@@ -498,7 +502,7 @@ torch::Tensor embed_fwd(torch::Tensor ids, torch::Tensor table, double scale, to
     const int each = wide ? kLookup<kPackSize<T, true>> : kLookup<1>;
     int lanes = 32;
     while (lanes < kThreads && lanes * each < packs) lanes <<= 1;
-    const unsigned blocks = static_cast<unsigned>(std::min<long>(blocks_for(tokens, kThreads / lanes), 1L << 30));
+    const unsigned blocks = static_cast<unsigned>(std::min<long>(blocks_for(tokens, kThreads / lanes), 148 * kLookupBlocks));
     (wide ? embed_fwd_kernel<T, true> : embed_fwd_kernel<T, false>)<<<blocks, kThreads, 0,
                                                                       at::cuda::getCurrentCUDAStream()>>>(
         flat.data_ptr<int64_t>(), tokens, rows.size(0), reinterpret_cast<const T*>(rows.data_ptr()), rows.stride(0), H,
