@@ -1,6 +1,9 @@
 // Python bindings of the sm_100a kernel library (module graspo_b200._C).
 #include <torch/extension.h>
 
+#include <stdexcept>
+#include <vector>
+
 namespace gb {
 bool& pdl_enabled();
 void gemm_tc(torch::Tensor A, torch::Tensor B, c10::optional<torch::Tensor> A2,
@@ -107,10 +110,21 @@ torch::Tensor embed_bwd(torch::Tensor dy, torch::Tensor ids, int64_t vocab, c10:
 std::vector<torch::Tensor> layer_norm_fwd(torch::Tensor x, torch::Tensor w, c10::optional<torch::Tensor> b, double eps);
 std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w, torch::Tensor mean,
                                           torch::Tensor rstd, bool bias32, torch::Tensor err);
-torch::Tensor grad_norm(std::vector<torch::Tensor> grads, int64_t device);
-torch::Tensor grad_clip(std::vector<torch::Tensor> grads, std::vector<torch::Tensor> out, double max_norm,
-                        int64_t device);
+using TensorRefs = std::vector<const torch::Tensor*>;
+torch::Tensor grad_norm(const TensorRefs& grads, int64_t device);
+torch::Tensor grad_clip(const TensorRefs& grads, const TensorRefs& out, double max_norm, int64_t device);
 }  // namespace gb
+
+// The tensors of a Python list, which holds them during the call.
+static gb::TensorRefs tensor_refs(const py::list& list) {
+  gb::TensorRefs refs;
+  refs.reserve(list.size());
+  for (const py::handle item : list) {
+    if (!THPVariable_Check(item.ptr())) throw std::invalid_argument("a list of tensors is wanted");
+    refs.push_back(&THPVariable_Unpack(item.ptr()));
+  }
+  return refs;
+}
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "graspo_b200 sm_100a kernels";
@@ -210,8 +224,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_bwd", &gb::layer_norm_bwd, "gradients of layer norm for x, weight and bias", py::arg("dy"),
         py::arg("x"), py::arg("w"), py::arg("mean"), py::arg("rstd"), py::arg("bias32"),
         py::arg("err"));
-  m.def("grad_norm", &gb::grad_norm, "global 2-norm of many tensors", py::arg("grads"),
-        py::arg("device"));
-  m.def("grad_clip", &gb::grad_clip, "scale many tensors to a global 2-norm of at most max_norm", py::arg("grads"),
-        py::arg("out"), py::arg("max_norm"), py::arg("device"));
+  m.def("grad_norm", [](const py::list& grads, int64_t device) { return gb::grad_norm(tensor_refs(grads), device); },
+        "global 2-norm of many tensors", py::arg("grads"), py::arg("device"));
+  m.def("grad_clip",
+        [](const py::list& grads, const py::list& out, double max_norm, int64_t device) {
+          return gb::grad_clip(tensor_refs(grads), tensor_refs(out), max_norm, device);
+        },
+        "scale many tensors to a global 2-norm of at most max_norm", py::arg("grads"), py::arg("out"),
+        py::arg("max_norm"), py::arg("device"));
 }

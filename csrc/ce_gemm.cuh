@@ -56,6 +56,7 @@ struct Args {
   int kb_first;           // kDh: K-blocks of the first piece, which fix the slices
   bool add;               // kDh: a later piece
   const float* unit;      // kDw: what the ratios are multiples of
+  bool early;             // host: how the kernel is launched
 };
 
 // Slices that the reduction of dh is split into, none of them empty: as many as
@@ -184,6 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmB);
   }
   if (warp == 1) tmem_alloc(tmem_slot, TileCfg::TMEM_COLS);
+  pdl_trigger();
   pdl_wait();
   const int live = __ldcg(args.live);
   const int M = MODE == kDw ? args.M : min(args.M, live);
@@ -429,6 +431,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Launches a kernel of the loss's chain.  `early`: it may start while its
+// predecessor runs; it comes up beside it and waits in pdl_wait().  Every kernel of
+// the chain calls pdl_wait() before it touches memory, in every thread, so that the
+// end of one implies the end of all before it.  Between kernels of some 8 us the
+// gaps were a fifth of the time (61 tokens x 512 x 4096: 51 us without, 40 with); at
+// 6144 x 4096 x 151936 the waiting blocks take up room that the running kernel's last
+// tiles share (25.9 ms without, 28.4 with), and at 466 x 1000 x 50001 it made no
+// difference.  kEarlyWork lies in between.
+constexpr double kEarlyWork = 4e9;   // tokens x vocabulary x hidden
+
+template <typename... KArgs, typename... A>
+void launch_chained(bool early, void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+}
+
 template <int MODE, int LAYOUT>
 void launch(const CUtensorMap& a, const CUtensorMap& b, const Args& args, cudaStream_t stream, int device) {
   auto kern = ce_gemm_kernel<MODE, LAYOUT>;
@@ -444,8 +471,7 @@ void launch(const CUtensorMap& a, const CUtensorMap& b, const Args& args, cudaSt
   // kDh splits by the grid's size: always one CTA per SM.  The others need no more than their tiles.
   const long tiles = static_cast<long>((args.M + BM - 1) / BM) * ((args.N + BN - 1) / BN);
   const int grid = MODE == kDh ? num_sms(device) : static_cast<int>(std::min<long>(tiles, num_sms(device)));
-  kern<<<grid, kThreads, smem, stream>>>(a, b, args);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_chained(args.early, kern, grid, kThreads, smem, stream, a, b, args);
 }
 
 }  // namespace ce

@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(kBlock) ce_compact_kernel(const int64_t* __res
                                                               int H, State st, float* __restrict__ loss,
                                                               __nv_bfloat16* __restrict__ out, int ldo,
                                                               int* __restrict__ err) {
+  pdl_trigger();
   __shared__ int own[kTokens];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long first = static_cast<long>(blockIdx.x) * kTokens;
@@ -148,6 +149,8 @@ __global__ void __launch_bounds__(kBlock) ce_compact_kernel(const int64_t* __res
 template <bool WIDE>
 __global__ void __launch_bounds__(kBlock) ce_pad_kernel(const __nv_bfloat16* __restrict__ in, long ldi, int H,
                                                           long rows, __nv_bfloat16* __restrict__ out, int ldo) {
+  pdl_trigger();
+  pdl_wait();
   for (long r = blockIdx.x * (kBlock / 32L) + (threadIdx.x >> 5); r < rows; r += gridDim.x * (kBlock / 32L))
     copy_row<WIDE>(in + r * ldi, H, out + r * ldo, ldo);
 }
@@ -162,6 +165,8 @@ __device__ __forceinline__ float common_weight(const float* g, bool mean, int n)
 __global__ void __launch_bounds__(kBlock) ce_finish_kernel(const float2* __restrict__ part, int parts, State st,
                                                              const float* __restrict__ g, bool mean,
                                                              float* __restrict__ loss) {
+  pdl_trigger();
+  pdl_wait();
   const int n = *st.count;
   const int lane = threadIdx.x & 31;
   if (blockIdx.x == 0 && threadIdx.x == 0) *st.unit = common_weight(g, mean, n);
@@ -190,6 +195,8 @@ __global__ void __launch_bounds__(kBlock) ce_finish_kernel(const float2* __restr
 // Unit and ratios from an upstream gradient per token (the unit is the largest
 // finite size, 1 where there is none), or the unit of a reduced loss.
 __global__ void __launch_bounds__(1024) ce_weight_kernel(const float* __restrict__ g, bool per_token, bool mean, State st) {
+  pdl_trigger();
+  pdl_wait();
   __shared__ float part[32];
   const int n = *st.count;
   if (!per_token) {
@@ -230,6 +237,8 @@ __device__ void total_loss(const float* __restrict__ loss, long T, int n, bool m
 
 __global__ void __launch_bounds__(kBlock) ce_total_kernel(const float* __restrict__ loss, long T, State st, bool mean,
                                                             float* __restrict__ out) {
+  pdl_trigger();
+  pdl_wait();
   total_loss(loss, T, *st.count, mean, out);
 }
 
@@ -241,6 +250,8 @@ __global__ void __launch_bounds__(kBlock) ce_scatter_kernel(const float* __restr
                                                               __nv_bfloat16* __restrict__ dh,
                                                               const float* __restrict__ loss, bool mean,
                                                               float* __restrict__ total) {
+  pdl_trigger();
+  pdl_wait();
   constexpr int V = WIDE ? 8 : 1;
   const int n = *st.count;
   const int row_blocks = gridDim.x - (total != nullptr ? 1 : 0);
@@ -305,6 +316,10 @@ void require(bool ok, const char* what) {
 
 enum Reduction : int64_t { kNone = 0, kSum = 1, kMean = 2 };
 
+bool launches_early(int64_t cap, int64_t V, int64_t H) {
+  return static_cast<double>(cap) * static_cast<double>(V) * static_cast<double>(H) < ce::kEarlyWork;
+}
+
 struct Forward {
   torch::Tensor loss, hc, state, W;   // loss per token; W as TMA reads it
   int64_t T, H, V, cap, Hp;
@@ -333,6 +348,7 @@ Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Ten
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   f.W = tma_rows(W, f.T, stream);
   ce::Args args{};
+  args.early = launches_early(f.cap, f.V, f.H);
   args.M = static_cast<int>(f.cap);
   args.N = static_cast<int>(f.V);
   args.kb = static_cast<int>((f.H + BK - 1) / BK);
@@ -343,9 +359,9 @@ Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Ten
   args.target_logit = st.target_logit;
   ce::launch<ce::kLse, 0>(make_tmap_bf16(f.hc.data_ptr(), f.cap, f.Hp, f.Hp, BM),
                           make_tmap_bf16(f.W.data_ptr(), f.V, f.H, f.W.stride(0), ce::BN), args, stream, device);
-  ce_finish_kernel<<<static_cast<int>(std::min<int64_t>((f.cap + 7) / 8, 148 * 8)), kBlock, 0, stream>>>(
-      args.part, 2 * num_n, st, grad, reduction == kMean, f.loss.data_ptr<float>());
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  ce::launch_chained(args.early, ce_finish_kernel, static_cast<unsigned>(std::min<int64_t>((f.cap + 7) / 8, 148 * 8)), kBlock, 0,
+                     stream, static_cast<const float2*>(args.part), 2 * num_n, st, grad, reduction == kMean,
+                     f.loss.data_ptr<float>());
   return f;
 }
 
@@ -355,6 +371,7 @@ void backward(const torch::Tensor& hc, const State& st, const torch::Tensor& W, 
               torch::Tensor* total, int* err, cudaStream_t stream) {
   const int device = hc.get_device();
   const int64_t cap = hc.size(0), Hp = hc.size(1);
+  const bool early = launches_early(cap, V, H);
   // A piece of d is at most 256 MiB: large enough that the three products of a
   // piece run for many waves of tiles, small against the logits.
   if (piece == 0) piece = std::max<int64_t>((256LL << 20) / (cap * 2) / ce::BN * ce::BN, ce::BN);
@@ -372,6 +389,7 @@ void backward(const torch::Tensor& hc, const State& st, const torch::Tensor& W, 
     const int64_t nv = std::min(piece, V - v0);
     const __nv_bfloat16* Wv = ptr<__nv_bfloat16>(W) + v0 * W.stride(0);
     ce::Args args{};
+    args.early = early;
     args.M = static_cast<int>(cap);
     args.N = static_cast<int>(nv);
     args.kb = static_cast<int>((H + BK - 1) / BK);
@@ -408,12 +426,12 @@ void backward(const torch::Tensor& hc, const State& st, const torch::Tensor& W, 
   }
   if (dh != nullptr) {
     const int rows = static_cast<int>(std::max<int64_t>(std::min<int64_t>(T, 148 * 16), 1));
-    (H % 8 == 0 ? ce_scatter_kernel<true> : ce_scatter_kernel<false>)
-        <<<rows + (total != nullptr ? 1 : 0), kBlock, 0, stream>>>(
-            acc.data_ptr<float>(), static_cast<int>(Hp), st, T, static_cast<int>(H), kb_first, sms,
-            ptr<__nv_bfloat16>(*dh), loss.defined() ? loss.data_ptr<float>() : nullptr, mean,
-            total != nullptr ? total->data_ptr<float>() : nullptr);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    ce::launch_chained(early, H % 8 == 0 ? ce_scatter_kernel<true> : ce_scatter_kernel<false>,
+                       rows + (total != nullptr ? 1 : 0), kBlock, 0, stream,
+                       static_cast<const float*>(acc.data_ptr<float>()), static_cast<int>(Hp), st, static_cast<long>(T),
+                       static_cast<int>(H), kb_first, sms, ptr<__nv_bfloat16>(*dh),
+                       static_cast<const float*>(loss.defined() ? loss.data_ptr<float>() : nullptr), mean,
+                       total != nullptr ? total->data_ptr<float>() : nullptr);
   }
 }
 
@@ -500,8 +518,7 @@ std::vector<torch::Tensor> ce_grads(torch::Tensor h, torch::Tensor W, torch::Ten
                             stream);
   const State st(f.state, f.cap);
   if (reduction == kNone && g != nullptr) {
-    ce_weight_kernel<<<1, 1024, 0, stream>>>(g, true, false, st);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    ce::launch_chained(launches_early(f.cap, f.V, f.H), ce_weight_kernel, 1, 1024, 0, stream, g, true, false, st);
   }
   torch::Tensor dh = torch::empty(h.sizes(), h.options()), dW, total;
   if (want_w) dW = torch::empty({f.V, f.H}, h.options());

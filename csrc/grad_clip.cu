@@ -29,6 +29,10 @@
 
 namespace gb {
 
+// The caller's tensors, which it keeps through the call (bindings.cpp): hundreds of
+// them, so no handle is copied.
+using TensorRefs = std::vector<const torch::Tensor*>;
+
 namespace {
 
 constexpr int kChunk = 4096;         // values; what the stretches are cut at
@@ -252,13 +256,13 @@ void require(bool ok, const char* what) {
 }
 
 // Entries of the tensors that hold values.
-std::vector<GradEntry> entries(const std::vector<torch::Tensor>& in, const std::vector<torch::Tensor>* out,
+std::vector<GradEntry> entries(const TensorRefs& in, const TensorRefs* out,
                                const torch::Tensor& like) {
   std::vector<GradEntry> v;
   v.reserve(in.size());
   const auto device = like.device();
   for (size_t i = 0; i < in.size(); ++i) {
-    const torch::Tensor& t = in[i];
+    const torch::Tensor& t = *in[i];
     require(t.device() == device && t.is_contiguous(), "gradients must be contiguous and on one device");
     GradEntry e{};
     e.in = t.data_ptr();
@@ -266,7 +270,7 @@ std::vector<GradEntry> entries(const std::vector<torch::Tensor>& in, const std::
     e.tin = e.tout = grad_type(t);
     e.out = const_cast<void*>(e.in);
     if (out != nullptr) {
-      const torch::Tensor& o = (*out)[i];
+      const torch::Tensor& o = *(*out)[i];
       require(o.device() == device && o.is_contiguous() && o.sizes() == t.sizes(),
               "outputs must be contiguous, on the gradients' device and of their shapes");
       e.out = o.data_ptr();
@@ -338,7 +342,7 @@ torch::Tensor norm_on(int64_t device) {
 }  // namespace
 
 // 2-norm of all values; `device` where there are no tensors to tell it.
-torch::Tensor grad_norm(std::vector<torch::Tensor> grads, int64_t device) {
+torch::Tensor grad_norm(const TensorRefs& grads, int64_t device) {
   torch::Tensor norm = norm_on(device);
   const c10::cuda::CUDAGuard guard(norm.device());
   auto stream = at::cuda::getCurrentCUDAStream();
@@ -349,8 +353,7 @@ torch::Tensor grad_norm(std::vector<torch::Tensor> grads, int64_t device) {
 }
 
 // out: empty to scale the gradients in place.
-torch::Tensor grad_clip(std::vector<torch::Tensor> grads, std::vector<torch::Tensor> out, double max_norm,
-                        int64_t device) {
+torch::Tensor grad_clip(const TensorRefs& grads, const TensorRefs& out, double max_norm, int64_t device) {
   require(out.empty() || out.size() == grads.size(), "one output per gradient");
   require(max_norm >= 0, "max_norm must not be negative");
   torch::Tensor norm = norm_on(device);

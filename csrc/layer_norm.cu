@@ -791,7 +791,7 @@ NormPlan bwd_plan(int H) {
     if constexpr (sizeof(T) == 4)
       if (packs <= 2048) return {&ln_bwd_kernel<T, V, 4, 1>, threads_for(packs, 4), 1};
   } else {
-    if (packs <= 1024) return {&ln_bwd_kernel<T, V, 2, 8>, threads_for(packs, 2), 2};
+    if (packs <= 1024) return {&ln_bwd_kernel<T, V, 4, 4>, threads_for(packs, 4), 2};
     if (packs <= 4096) return {&ln_bwd_kernel<T, V, 8, 2>, threads_for(packs, 8), 1};
     if (packs <= 8192) return {&ln_bwd_kernel<T, V, 16, 1>, threads_for(packs, 16), 1};
   }

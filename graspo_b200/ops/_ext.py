@@ -60,18 +60,15 @@ launches = LaunchCounter()
 class _Counting:
     def __init__(self, module) -> None:
         self._module = module
-        self._cache: dict[str, object] = {}
 
     def __getattr__(self, name: str):
-        fn = self._cache.get(name)
-        if fn is None:
-            raw = getattr(self._module, name)
+        raw = getattr(self._module, name)
 
-            def fn(*args, _raw=raw, **kwargs):
-                launches.count += 1
-                return _raw(*args, **kwargs)
+        def fn(*args, _raw=raw, **kwargs):
+            launches.count += 1
+            return _raw(*args, **kwargs)
 
-            self._cache[name] = fn
+        self.__dict__[name] = fn  # found without this call from now on
         return fn
 
 
