@@ -135,8 +135,11 @@ __device__ __forceinline__ void store_chunk(__nv_bfloat16* C, const float (&v)[3
 // The warp's 32 rows x 32 values, row per lane, to 32 rows of C (the lane's first
 // value at C, rows ldc apart) through 2 KB of shared memory, so that an access
 // covers 8 rows of 64 bytes instead of 32 of 16: with a row per lane the stores
-// of dW took as many cycles in L1 as 8 K-blocks of products.
-__device__ __forceinline__ void store_rows(uint8_t* stage, __nv_bfloat16* C, long ldc, const float (&v)[32], int rows) {
+// of dW took as many cycles in L1 as 8 K-blocks of products.  Rows that start off a
+// 16-byte boundary (`wide` false), and the last columns, are written a row at a time,
+// a value per lane.
+__device__ __forceinline__ void store_rows(uint8_t* stage, __nv_bfloat16* C, long ldc, const float (&v)[32], int rows,
+                                           int count, bool wide) {
   const int lane = threadIdx.x & 31;
   uint4* s = reinterpret_cast<uint4*>(stage);
   __syncwarp();
@@ -146,11 +149,18 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, __nv_bfloat16* C, lon
         make_uint4(bf16_pair(v[8 * q], v[8 * q + 1]), bf16_pair(v[8 * q + 2], v[8 * q + 3]),
                    bf16_pair(v[8 * q + 4], v[8 * q + 5]), bf16_pair(v[8 * q + 6], v[8 * q + 7]));
   __syncwarp();
+  if (wide && count >= 32) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2), q = lane & 3;
-    const uint4 x = s[r * 4 + (q ^ ((r >> 1) & 3))];
-    if (r < rows) reinterpret_cast<uint4*>(C + r * ldc)[q] = x;
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2), q = lane & 3;
+      const uint4 x = s[r * 4 + (q ^ ((r >> 1) & 3))];
+      if (r < rows) reinterpret_cast<uint4*>(C + r * ldc)[q] = x;
+    }
+  } else {
+    const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(stage);
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (r < rows && lane < count) C[r * ldc + lane] = h[r * 32 + ((lane >> 3) ^ ((r >> 1) & 3)) * 8 + (lane & 7)];
   }
 }
 
@@ -407,13 +417,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= unit;
             __nv_bfloat16* C = static_cast<__nv_bfloat16*>(args.C) + nc;
-            if (count >= 32 && align >= 16) {
-              // the 16 KB past the stages belong to the epilogue's warps
-              store_rows(smem + STAGES * TileCfg::STAGE_BYTES + 256 + (warp - 2) * 2048, C + (m - lane) * args.ldc,
-                         args.ldc, v, M - (m - lane));
-            } else if (m < M) {
-              store_chunk(C + m * args.ldc, v, count, align);
-            }
+            // the 16 KB past the stages and barriers belong to the epilogue's warps
+            store_rows(smem + STAGES * TileCfg::STAGE_BYTES + 256 + (warp - 2) * 2048, C + (m - lane) * args.ldc,
+                       args.ldc, v, M - (m - lane), count, align >= 16);
           }
         }
         tc_fence_before();

@@ -86,21 +86,40 @@ __device__ __forceinline__ int block_sum(int v) {
 }
 
 // Row of `in` to row of `out`, zeros in the columns [H, ldo); zeros without `in`.
+// Rows of `out` are whole 128-byte lines; those of `in` that are not on 16-byte
+// boundaries are read value by value, eight in flight.
 template <bool WIDE>
 __device__ __forceinline__ void copy_row(const __nv_bfloat16* in, int H, __nv_bfloat16* out, int ldo) {
-  constexpr int V = WIDE ? 8 : 1;
+  const int lane = threadIdx.x & 31;
+  if constexpr (WIDE) {
 #pragma unroll 4
-  for (int c = (threadIdx.x & 31) * V; c < ldo; c += 32 * V) {
-    Pack<__nv_bfloat16, V> p = {};
-    if (in != nullptr && c < H) p = load_raw<__nv_bfloat16, V>(in + c);
-    store_raw<__nv_bfloat16, V>(out + c, p);
+    for (int c = lane * 8; c < ldo; c += 256) {
+      Pack<__nv_bfloat16, 8> p = {};
+      if (in != nullptr && c < H) p = load_raw<__nv_bfloat16, 8>(in + c);
+      store_raw<__nv_bfloat16, 8>(out + c, p);
+    }
+  } else {
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(in);
+    for (int c0 = 0; c0 < ldo; c0 += 256) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + i * 64 + lane * 2;
+        const uint32_t lo = in != nullptr && c < H ? src[c] : 0u, hi = in != nullptr && c + 1 < H ? src[c + 1] : 0u;
+        w[i] = hi << 16 | lo;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c0 + i * 64 + lane * 2 < ldo) *reinterpret_cast<uint32_t*>(out + c0 + i * 64 + lane * 2) = w[i];
+    }
   }
 }
 
 // The trained tokens' rows of h, one after the other, and their places.  A block
 // counts the trained tokens before its own 32 itself: 8 bytes a token from L2
 // against some 10 ns of products, and no second pass.  The last block knows the
-// count and zeroes the rows that fill the last tile.  A target outside the
+// count and zeroes the rows that fill the last K-block of dW (what the rest of the
+// last tile holds stays in its own rows).  A target outside the
 // vocabulary that is not ignore_index is reported in err[1] and gets a NaN loss
 // and a zero gradient.
 template <bool WIDE>
@@ -140,7 +159,7 @@ __global__ void __launch_bounds__(kBlock) ce_compact_kernel(const int64_t* __res
   if (blockIdx.x == gridDim.x - 1) {
     const int total = before + count;
     if (threadIdx.x == 0) *st.count = total;
-    for (long m = total + warp; m < (total + kRowPad - 1) / kRowPad * kRowPad; m += kBlock / 32)
+    for (long m = total + warp; m < (total + BK - 1) / BK * BK; m += kBlock / 32)
       copy_row<WIDE>(nullptr, H, out + m * ldo, ldo);
   }
 }
@@ -262,24 +281,26 @@ __global__ void __launch_bounds__(kBlock) ce_scatter_kernel(const float* __restr
   const float unit = *st.unit;
   const int slices = ce::dh_slices(n, H, kb_first, sms);
   const long slice = ce::dh_slice_elements(n, lda);
-  for (long t = blockIdx.x; t < T; t += row_blocks) {
+  const int per_row = (H + kBlock * V - 1) / (kBlock * V);  // blocks' columns
+  for (long i = blockIdx.x; i < T * per_row; i += row_blocks) {
+    const long t = i / per_row;
+    const int c = static_cast<int>(i - t * per_row) * kBlock * V + threadIdx.x * V;
     const int m = st.place[t];
-    for (int c = threadIdx.x * V; c < H; c += kBlock * V) {
-      float s[V] = {};
-      if (m >= 0) {
-        const float* src = acc + static_cast<long>(m) * lda + c;
-#pragma unroll 4
-        for (int k = 0; k < slices; ++k) {
-          float f[V];
-          load_pack<float, V>(src + k * slice, f);
+    if (c >= H) continue;
+    float s[V] = {};
+    if (m >= 0) {
+      const float* src = acc + static_cast<long>(m) * lda + c;
+#pragma unroll 8
+      for (int k = 0; k < slices; ++k) {
+        float f[V];
+        load_pack<float, V>(src + k * slice, f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) s[i] += f[i];
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) s[i] *= unit;
+        for (int j = 0; j < V; ++j) s[j] += f[j];
       }
-      store_pack<__nv_bfloat16, V>(dh + t * H + c, s);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] *= unit;
     }
+    store_pack<__nv_bfloat16, V>(dh + t * H + c, s);
   }
 }
 
@@ -425,7 +446,8 @@ void backward(const torch::Tensor& hc, const State& st, const torch::Tensor& W, 
     }
   }
   if (dh != nullptr) {
-    const int rows = static_cast<int>(std::max<int64_t>(std::min<int64_t>(T, 148 * 16), 1));
+    const int64_t per_row = (H + kBlock * (H % 8 == 0 ? 8 : 1) - 1) / (kBlock * (H % 8 == 0 ? 8 : 1));
+    const int rows = static_cast<int>(std::max<int64_t>(std::min<int64_t>(T * per_row, 148 * 16), 1));
     ce::launch_chained(early, H % 8 == 0 ? ce_scatter_kernel<true> : ce_scatter_kernel<false>,
                        rows + (total != nullptr ? 1 : 0), kBlock, 0, stream,
                        static_cast<const float*>(acc.data_ptr<float>()), static_cast<int>(Hp), st, static_cast<long>(T),
