@@ -134,7 +134,7 @@ struct NormArgs {
 };
 
 template <typename T, int V, int VPT, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kFewRows, BLOCK ? 1 : 8) ln_fwd_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kFewRows, BLOCK ? 2 : 8) ln_fwd_kernel(const NormArgs a) {
   __shared__ float scratch[32];
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31;
   const int width = BLOCK ? blockDim.x : 32;
