@@ -5,7 +5,8 @@
 // device (the number of trained tokens) and whose epilogues are the loss's.
 //
 //   kCeLse    rows tokens, columns vocabulary.  Per row and half tile of 128
-//             columns (max, sum of exp); the logit of the row's target.
+//             columns (max, sum of exp) without the row's target; the target's
+//             logit by itself.
 //   kCeGrad   the same product; d = r (exp(l - lse) - [v = y]) in bf16.
 //   kCeDh     rows tokens, columns hidden, K a vocabulary piece: fp32 sums of
 //             dh, K split into slices where there are few tiles.
@@ -349,6 +350,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(&tempty[acc]);
         }
         const int count = args.N - n0;  // columns that exist
+        if (m < M && target >= 0 && target < 128) {  // the target is not among the others
+#pragma unroll
+          for (int j = 0; j < 128; ++j)
+            if (target == j) {
+              args.target_logit[m] = logit[j];
+              logit[j] = -INFINITY;
+            }
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 128; ++j) {
@@ -360,15 +369,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         float s[4] = {};
 #pragma unroll
         for (int j = 0; j < 128; ++j) s[j & 3] += ex2(fmaf(logit[j], kLog2e, -base));
-        if (m < M) {
+        if (m < M)
           args.part[static_cast<long>(m) * (2 * num_n) + 2 * w.n_block + half] =
               make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
-          if (target >= 0 && target < 128) {
-#pragma unroll
-            for (int j = 0; j < 128; ++j)
-              if (target == j) args.target_logit[m] = logit[j];
-          }
-        }
       } else {
         const int acc = acc_iter & 1;
         const bool have = mbar_wait(&tfull[acc], (acc_iter >> 1) & 1, args.err, kErrTmemFullTimeout);

@@ -415,9 +415,11 @@ def ce_forward(h, W, targets, ignore_index, reduction, err):
     hc = h.reshape(-1, h.shape[-1])[rows]
     logits = _f(hc) @ _f(W).T
     lse = torch.logsumexp(logits, -1)
+    lead = logits - logits.gather(1, t[rows, None])
+    lead.scatter_(1, t[rows, None], -math.inf)
     loss = torch.zeros(t.shape)
     loss[bad] = float("nan")
-    loss[rows] = lse - logits.gather(1, t[rows, None])[:, 0]
+    loss[rows] = torch.logaddexp(torch.zeros(()), torch.logsumexp(lead, -1))
     state = torch.stack([rows.double(), t[rows].double(), lse.double()])
     if reduction == 0:
         return loss.view(targets.shape), hc, state

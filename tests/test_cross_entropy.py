@@ -11,6 +11,7 @@ error (relative 3 delta + 2^-17) and one rounding to bf16 (8 significant bits:
 2^-8); dh and dW sum entries with those errors and are rounded to bf16 once more.
 """
 
+import contextlib
 import math
 
 import pytest
@@ -316,3 +317,66 @@ def test_refusals_on_the_gpu():
         linear_cross_entropy(h, w, t.cpu())
     with pytest.raises(ValueError):
         linear_cross_entropy_grads(h, w, t, piece=100)
+
+
+def _confident(T, H, V, offset, device):
+    """Tokens whose target leads by 6 to 20 (losses of 1e-1 down to 1e-6), all logits shifted by `offset`."""
+    g = torch.Generator().manual_seed(H + offset)
+    u = torch.randn(H, generator=g)
+    u /= u.norm()
+    w = torch.randn(V, H, generator=g) * (2.0 / math.sqrt(H))
+    w += (2.0 - w @ u)[:, None] * u                          # every row has the same part along u
+    t = torch.randint(0, V, (T,), generator=g)
+    lead = torch.linspace(1.5, 5.0, T)[:, None] * (w[t] - 2.0 * u)
+    h = lead + (offset / 2.0) * u
+    return h.to(device, torch.bfloat16), w.to(device, torch.bfloat16), t.to(device)
+
+
+def _confident_oracle(h, w, t):
+    """Logits' error delta as above, and loss, others' share R of each target's and 64-bit logits.  The loss is
+    log(1 + R) with R = sum exp(l_v - l_y) over the others: two logits' errors and the exponentials' (2^-16 with the
+    roundings of the exponent, at most 32 here) are errors relative to the loss itself."""
+    logits = h.double() @ w.double().T
+    at = t[:, None]
+    lead = logits - logits.gather(1, at)
+    share = torch.exp(lead.scatter(1, at, -torch.inf))
+    delta = (h.shape[1] / 16 + 16) * 2.0 ** -22 * float((h.double().abs() @ w.double().abs().T).max())
+    return torch.log1p(share.sum(-1)), share, delta
+
+
+CONFIDENT = [(96, 4096, 515, 0), (96, 4096, 515, 300), (130, 64, 777, 40), (50, 1000, 300, -100)]
+
+
+@pytest.mark.parametrize("T,H,V,offset", CONFIDENT)
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_losses_of_confident_tokens(T, H, V, offset, device):
+    from graspo_b200.ops.cross_entropy import _LinearCrossEntropy
+    from graspo_b200.ops.emulate import use_emulation
+
+    h, w, t = _confident(T, H, V, offset, device)
+    want, _, delta = _confident_oracle(h, w, t)
+    assert float(want.min()) < 1e-5 and float(want.max()) > 1e-2
+    with use_emulation() if device == "cpu" else contextlib.nullcontext():
+        loss = _LinearCrossEntropy.apply(h, w, t, IGNORE, "none", 0)
+    _within(loss, want, want * (math.expm1(2 * delta) + 2.0 ** -16), "loss")
+
+
+@pytest.mark.gpu
+def test_infinite_logits():
+    """As log_softmax has it: an infinite logit leaves no loss (NaN) unless it is the target's and -inf (inf)."""
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy
+
+    w = torch.zeros(300, 64, device="cuda", dtype=torch.bfloat16)
+    w[:, 1] = torch.linspace(-1, 1, 300)
+    h = torch.ones(5, 64, device="cuda", dtype=torch.bfloat16)
+    t = torch.tensor([7, 299, 0, 150, 7], device="cuda")
+    for value, want in ((math.inf, [math.nan] * 5), (-math.inf, [math.inf, None, None, None, math.inf]),
+                        (math.nan, [math.nan] * 5)):
+        bad = w.clone()
+        bad[7, 0] = value
+        loss = linear_cross_entropy(h, bad, t, reduction="none")
+        logits = h.double() @ bad.double().T
+        ref = -torch.log_softmax(logits, -1).gather(1, t[:, None])[:, 0]
+        assert torch.equal(loss.isnan(), ref.isnan()) and torch.equal(loss.isinf(), ref.isinf())
+        for got, r, v in zip(loss.tolist(), ref.tolist(), want):
+            assert v is None and abs(got - r) < 1e-5 or v is not None and (got == v or got != got and v != v)
