@@ -7,7 +7,8 @@
 //   kCeLse    rows tokens, columns vocabulary.  Per row and half tile of 128
 //             columns (max, sum of exp) without the row's target; the target's
 //             logit by itself.
-//   kCeGrad   the same product; d = r (exp(l - lse) - [v = y]) in bf16.
+//   kCeGrad   the same product; d = r exp(l - lse) in bf16, and r (p - 1) from the
+//             forward's loss in the target's column.
 //   kCeDh     rows tokens, columns hidden, K a vocabulary piece: fp32 sums of
 //             dh, K split into slices where there are few tiles.
 //   kCeDw     rows vocabulary, columns hidden, K the tokens: dW in bf16.
@@ -21,8 +22,11 @@
 // The tensor cores truncate the running sum at every step of 16 products, which
 // shrinks a logit by some 1e-9 of itself per product: 4e-6 at H = 4096, seen as
 // 2.5e-5 in every loss.  kCeLse therefore takes the reduction in segments of
-// kSegment K-blocks and adds those in registers, round to nearest.  The other
-// products end in bf16, where 4e-6 is nothing.
+// kSegment K-blocks and adds those in registers, round to nearest.  kCeGrad does
+// without: an error of a logit is one relative to exp(l - lse), which is rounded to
+// bf16.  Only p - 1 cancels, and that is not made from the remade logit: it is
+// expm1(-loss), relatively as exact as the loss.  In the sums of kCeDh and kCeDw
+// the truncation is far below the bf16 of their operands.
 #include "gemm_tc.cuh"
 
 namespace gb {
@@ -49,6 +53,7 @@ struct Args {
   float2* part;           // [M][2 blocks]
   float* target_logit;
   const float* lse;
+  const float* hot;       // p - 1 of each token's target
   const float* ratio;     // r of each token
   int n_first;            // vocabulary index of column 0
   // results
@@ -322,12 +327,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (w.kb_end <= w.kb_begin) continue;
       long target = 0;
-      float lse2 = 0.f, ratio = 0.f;
+      float lse2 = 0.f, ratio = 0.f, hot_d = 0.f;
       if (m < M) {
         if constexpr (MODE == kLse || MODE == kGrad) target = args.target[m] - args.n_first - n0;
         if constexpr (MODE == kGrad) {
           lse2 = args.lse[m] * kLog2e;
           ratio = args.ratio[m];
+          hot_d = ratio * args.hot[m];
         }
       }
       if constexpr (MODE == kLse) {
@@ -386,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (m < M) {
               const int hot = static_cast<int>(target) - c * 32;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = ratio * (ex2(fmaf(v[j], kLog2e, -lse2)) - (j == hot ? 1.f : 0.f));
+              for (int j = 0; j < 32; ++j) v[j] = j == hot ? hot_d : ratio * ex2(fmaf(v[j], kLog2e, -lse2));
               store_chunk(C, v, count, align);
             } else if (m < (M + BK - 1) / BK * BK) {
               // dW contracts over whole blocks of BK tokens: the rows that fill the last one are zero

@@ -58,6 +58,7 @@ struct State {
   float* lse;
   float* ratio;         // its weight over the unit
   float* target_logit;
+  float* hot;           // p - 1 of its target
   static int64_t words(int64_t cap) { return 4 + 8 * cap; }
   State(const torch::Tensor& t, int64_t cap) {
     int* p = t.data_ptr<int>();
@@ -69,6 +70,7 @@ struct State {
     lse = reinterpret_cast<float*>(place + cap);
     ratio = lse + cap;
     target_logit = ratio + cap;
+    hot = target_logit + cap;
   }
 };
 
@@ -188,7 +190,8 @@ __device__ __forceinline__ float common_weight(const float* g, bool mean, int n)
 // reduced loss.  With z = log sum exp(others) - t the loss is log(1 + e^z): exact
 // relative to itself however small it is.  (lse - t, both rounded first, has steps
 // of the largest logit's last place, 2e-6 at 20 and 3e-5 at 300, where a confident
-// token's loss is 1e-6.)
+// token's loss is 1e-6.)  p - 1 = expm1(-loss) likewise: exp(l - lse) - 1 from the
+// remade logit was off by 2.5e-5, a quarter of it at a loss of 1e-4.
 __global__ void __launch_bounds__(kBlock) ce_finish_kernel(const float2* __restrict__ part, int parts, State st,
                                                              const float* __restrict__ g, bool mean,
                                                              float* __restrict__ loss) {
@@ -218,7 +221,9 @@ __global__ void __launch_bounds__(kBlock) ce_finish_kernel(const float2* __restr
       const bool lost = t == INFINITY;
       st.lse[m] = lost ? __int_as_float(0x7fc00000) : z > 0.f ? (top + rest) + q : t + q;
       st.ratio[m] = 1.f;
-      loss[st.token[m]] = lost ? __int_as_float(0x7fc00000) : fmaxf(z, 0.f) + q;
+      const float l = lost ? __int_as_float(0x7fc00000) : fmaxf(z, 0.f) + q;
+      st.hot[m] = expm1f(-l);
+      loss[st.token[m]] = l;
     }
   }
 }
@@ -430,6 +435,7 @@ void backward(const torch::Tensor& hc, const State& st, const torch::Tensor& W, 
     args.err = err;
     args.target = st.target;
     args.lse = st.lse;
+    args.hot = st.hot;
     args.ratio = st.ratio;
     args.n_first = static_cast<int>(v0);
     args.C = d.data_ptr();

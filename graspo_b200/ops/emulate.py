@@ -405,7 +405,7 @@ def _ce_live(targets, V, ignore_index):
 
 
 def ce_forward(h, W, targets, ignore_index, reduction, err):
-    """The state's tensors here are the trained rows and (position, target, lse) of each."""
+    """The state's tensors here are the trained rows and (position, target, lse, p - 1) of each."""
     t = targets.reshape(-1).long()
     live = _ce_live(t, W.shape[0], ignore_index)
     bad = ~live & (t != ignore_index)
@@ -420,7 +420,7 @@ def ce_forward(h, W, targets, ignore_index, reduction, err):
     loss = torch.zeros(t.shape)
     loss[bad] = float("nan")
     loss[rows] = torch.logaddexp(torch.zeros(()), torch.logsumexp(lead, -1))
-    state = torch.stack([rows.double(), t[rows].double(), lse.double()])
+    state = torch.stack([rows.double(), t[rows].double(), lse.double(), torch.expm1(-loss[rows]).double()])
     if reduction == 0:
         return loss.view(targets.shape), hc, state
     return loss.sum() / (max(1, rows.numel()) if reduction == 2 else 1), hc, state
@@ -436,8 +436,9 @@ def ce_backward(hc, state, W, tokens, grad, reduction, want_h, want_w, piece, er
     h, acc, dw = _f(hc), torch.zeros(n, H), torch.empty(V, H, dtype=hc.dtype)
     for v0 in range(0, V, piece or V):
         Wv = _f(W[v0 : v0 + (piece or V)])
-        hot = (target[:, None] == torch.arange(v0, v0 + Wv.shape[0])).float()
-        d = (ratio[:, None] * (torch.exp(h @ Wv.T - lse[:, None]) - hot)).to(hc.dtype).float()
+        hot = target[:, None] == torch.arange(v0, v0 + Wv.shape[0])
+        p = torch.where(hot, state[3].float()[:, None], torch.exp(h @ Wv.T - lse[:, None]))
+        d = (ratio[:, None] * p).to(hc.dtype).float()
         acc += d @ Wv
         dw[v0 : v0 + Wv.shape[0]] = (d.T @ h * unit).to(dw.dtype)
     dh = torch.zeros(tokens, H, dtype=hc.dtype)

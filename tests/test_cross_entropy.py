@@ -380,3 +380,28 @@ def test_infinite_logits():
         assert torch.equal(loss.isnan(), ref.isnan()) and torch.equal(loss.isinf(), ref.isinf())
         for got, r, v in zip(loss.tolist(), ref.tolist(), want):
             assert v is None and abs(got - r) < 1e-5 or v is not None and (got == v or got != got and v != v)
+
+
+@pytest.mark.parametrize("T,H,V,offset", CONFIDENT)
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_gradients_of_confident_tokens(T, H, V, offset, reduction, device):
+    """The target's entry of d is -(1 - p), whose error is relative to 1 - p and not to 1: every entry of dh and
+    dW within the logits' error and the rounding of d (2^-8) of sums over |p - hot|."""
+    from graspo_b200.ops.cross_entropy import _LinearCrossEntropy
+    from graspo_b200.ops.emulate import use_emulation
+
+    h, w, t = _confident(T, H, V, offset, device)
+    up = torch.randn(T, generator=torch.Generator().manual_seed(1)).to(device)
+    _, share, delta = _confident_oracle(h, w, t)
+    rest = share.sum(-1, keepdim=True)
+    d = (share / (1 + rest)).scatter(1, t[:, None], -rest / (1 + rest))
+    d = d * (up.double()[:, None] if reduction == "none" else 1 / T)
+    hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    with use_emulation() if device == "cpu" else contextlib.nullcontext():
+        loss = _LinearCrossEntropy.apply(hl, wl, t, IGNORE, reduction, 0)
+        loss.backward(up if reduction == "none" else None)
+    rel = (2.0 ** -8 + 4 * delta + 2.0 ** -16) * (1 + 2.0 ** -8)
+    wh, ww = d @ w.double(), d.T @ h.double()
+    _within(hl.grad, wh, rel * (d.abs() @ w.double().abs()) + 2.0 ** -8 * wh.abs() + 1e-30, "dh")
+    _within(wl.grad, ww, rel * (d.T.abs() @ h.double().abs()) + 2.0 ** -8 * ww.abs() + 1e-30, "dw")
