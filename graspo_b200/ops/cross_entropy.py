@@ -2,8 +2,9 @@
 
 ``linear_cross_entropy(h, weight, targets)`` is ``F.cross_entropy(h @ weight^T,
 targets)`` for hidden states ``h`` [..., H] and a projection ``weight`` [V, H],
-as an autograd function of both; ``linear_cross_entropy_grads`` returns the loss
-and both gradients at once for callers that run their backward by hand (as
+as an autograd function of both (on the GPU differentiable once: a second
+derivative raises); ``linear_cross_entropy_grads`` returns the loss and both
+gradients at once for callers that run their backward by hand (as
 ``models/fused.py`` does).
 
 * ``targets`` equal to ``ignore_index`` take no part: loss 0, gradient 0, and
@@ -29,6 +30,7 @@ from __future__ import annotations
 import torch
 
 from graspo_b200.ops._ext import err_word, ext, launches
+from graspo_b200.ops._second import edge_of, refuse_second
 
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
@@ -64,21 +66,27 @@ def _torch_loss(h, weight, targets, ignore_index, reduction):
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h, weight, targets, ignore_index, reduction, piece):
+    def forward(ctx, h, weight, targets, ignore_index, reduction, piece, h_edge=None):
         launches.add(2 + (reduction != "none"))      # compaction, product, row sums (and their total)
         loss, *state = ext().ce_forward(h, weight, targets, ignore_index, REDUCTIONS[reduction], err_word(h.device))
-        ctx.save_for_backward(weight, *state)
+        ctx.save_for_backward(weight, h_edge, *state)
         ctx.shape, ctx.tokens, ctx.reduction, ctx.piece = h.shape, targets.numel(), reduction, piece
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        weight, hc, state = ctx.saved_tensors
+        weight, h_edge, hc, state = ctx.saved_tensors
         launches.add(4)                              # weights, three products a piece, the rows of dh
         dh, dw = ext().ce_backward(hc, state, weight, ctx.tokens, g.float().contiguous().view(-1),
                                    REDUCTIONS[ctx.reduction], ctx.needs_input_grad[0], ctx.needs_input_grad[1],
                                    ctx.piece, err_word(hc.device))
-        return (None if dh is None else dh.view(ctx.shape)), dw, None, None, None, None
+        dh, dw = refuse_second("linear_cross_entropy", (None if dh is None else dh.view(ctx.shape), dw),
+                               g, weight, h_edge)
+        return dh, dw, None, None, None, None, None
+
+
+def _kernel_loss(h, weight, targets, ignore_index, reduction, piece):
+    return _LinearCrossEntropy.apply(h, weight, targets, ignore_index, reduction, piece, edge_of(h))
 
 
 def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
@@ -88,7 +96,7 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     ``piece``: vocabulary columns per piece of the backward (a multiple of 256;
     0 takes as many as 256 MiB of softmax gradients hold)."""
     if h.is_cuda and reduction in REDUCTIONS:
-        return _LinearCrossEntropy.apply(h, weight, targets, int(ignore_index), reduction, int(piece))
+        return _kernel_loss(h, weight, targets, int(ignore_index), reduction, int(piece))
     _check(h, weight, targets, reduction, piece)
     return _torch_loss(h, weight, targets, ignore_index, reduction)
 

@@ -1,9 +1,10 @@
 """Embedding lookup with a scale and a trained table (csrc/embedding_grad.cu).
 
 ``embedding(ids, table, scale=s)`` is ``s * table[ids]`` (one rounding),
-differentiable in ``table``; ``embedding_grad`` is its gradient for callers
-that run their backward by hand, written whole or added to a gradient that is
-there (a table that is also the vocabulary projection).
+differentiable in ``table`` (once: a second derivative raises);
+``embedding_grad`` is its gradient for callers that run their backward by hand,
+written whole or added to a gradient that is there (a table that is also the
+vocabulary projection).
 
 The gradient sorts the tokens by id and adds each row's tokens in fp32 in token
 order: the result does not depend on timing, whatever the repetitions, and is
@@ -20,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from graspo_b200.ops._ext import err_word, ext, launches
+from graspo_b200.ops._second import refuse_second
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _NO_ID = -(1 << 63)
@@ -99,7 +101,8 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
-        return None, embedding_grad(dy, ids, ctx.vocab, scale=ctx.scale, padding_idx=ctx.padding), None, None
+        grad = embedding_grad(dy, ids, ctx.vocab, scale=ctx.scale, padding_idx=ctx.padding)
+        return None, *refuse_second("embedding", (grad,), dy), None, None
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0,

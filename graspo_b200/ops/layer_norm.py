@@ -2,8 +2,9 @@
 
 ``layer_norm(x, weight, bias, eps)`` normalises the last dimension of ``x``
 (fp32 statistics, one rounding of the result) and is differentiable in all
-three; ``layer_norm_forward`` / ``layer_norm_backward`` are its two halves for
-callers that run their backward by hand.
+three (once: a second derivative raises); ``layer_norm_forward`` /
+``layer_norm_backward`` are its two halves for callers that run their backward by
+hand.
 
 ``x`` is bf16, fp16 or fp32 of any leading shape; weight and bias have its type
 or are fp32 (their gradients have the type of each).  ``bias`` may be None.
@@ -20,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from graspo_b200.ops._ext import err_word, ext, launches
+from graspo_b200.ops._second import refuse_second
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -90,7 +92,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         dx, dw, db = layer_norm_backward(dy, x, weight, mean, rstd, ctx.bias_dtype)
-        return dx, dw, None if ctx.bias_dtype is None else db, None
+        return *refuse_second("layer_norm", (dx, dw, None if ctx.bias_dtype is None else db), dy, x, weight), None
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,

@@ -405,3 +405,41 @@ def test_gradients_of_confident_tokens(T, H, V, offset, reduction, device):
     wh, ww = d @ w.double(), d.T @ h.double()
     _within(hl.grad, wh, rel * (d.abs() @ w.double().abs()) + 2.0 ** -8 * wh.abs() + 1e-30, "dh")
     _within(wl.grad, ww, rel * (d.T.abs() @ h.double().abs()) + 2.0 ** -8 * ww.abs() + 1e-30, "dw")
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_second_derivatives_are_refused(device, frozen):
+    """Also where the upstream gradient is a constant, and where a larger loss holds the term."""
+    from graspo_b200.ops.cross_entropy import _kernel_loss
+    from graspo_b200.ops.emulate import use_emulation
+
+    h, w, t, _ = _case(20, 64, 256, 1.0, device=device)
+    hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(not frozen)
+    leaves = (hl,) if frozen else (hl, wl)
+    with use_emulation() if device == "cpu" else contextlib.nullcontext():
+        loss = _kernel_loss(hl, wl, t, IGNORE, "mean", 0)
+        plain = torch.autograd.grad(loss, leaves, retain_graph=True)
+        grads = torch.autograd.grad(loss, leaves, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+        for second in grads:
+            for leaf in leaves:
+                with pytest.raises(RuntimeError, match="second derivative"):
+                    torch.autograd.grad(loss + second.float().square().sum(), leaf, retain_graph=True)
+        (loss + hl.float().sum()).backward()                 # nothing of a second order in it
+    assert hl.grad is not None
+
+
+def test_second_derivatives_of_the_cpu_form():
+    """The CPU form is PyTorch's own operations: differentiable twice."""
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy
+
+    h, w, t, _ = _case(9, 6, 11, 0.7, device="cpu")
+    both = []
+    for form in (lambda a, b: linear_cross_entropy(a, b, t),
+                 lambda a, b: torch.nn.functional.cross_entropy(a @ b.T, t, ignore_index=IGNORE)):
+        a, b = h.float().requires_grad_(True), w.float().requires_grad_(True)
+        da, db = torch.autograd.grad(form(a, b), (a, b), create_graph=True)
+        both.append(torch.autograd.grad(da.square().sum() + db.square().sum(), (a, b)))
+    for x, y in zip(*both):                                  # fp32 sums of at most 11 terms of order 1
+        assert (x - y).abs().max() < 64 * 2.0 ** -23

@@ -236,3 +236,17 @@ def test_refusals(device):
                 lambda: embedding_grad(dy, ids, 10, padding_idx=-1)]:
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_second_derivatives_are_refused(device):
+    from graspo_b200.ops.embedding import embedding
+
+    ids, table, dy = _case(6, 10, 8, torch.float32, device=device)
+    leaf, up = table.clone().requires_grad_(True), dy.clone().requires_grad_(True)
+    (grad,) = torch.autograd.grad(embedding(ids, leaf), leaf, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(up.sum() + grad.square().sum(), up, retain_graph=True)
+    # with a constant upstream gradient the table's does not depend on anything
+    (grad,) = torch.autograd.grad(embedding(ids, leaf), leaf, dy, create_graph=True)
+    assert not grad.requires_grad

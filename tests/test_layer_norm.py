@@ -260,3 +260,22 @@ def test_refusals(device):
                 lambda: layer_norm_backward(dy, x, w, mean[:2], rstd)]:
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_second_derivatives_are_refused(device):
+    """Also where the upstream gradient is a constant, and where a larger loss holds the term."""
+    from graspo_b200.ops.layer_norm import layer_norm
+
+    x, w, b, dy = _case(4, 16, torch.float32, device=device)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = layer_norm(*leaves)
+    plain = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    grads = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(plain, grads))
+    for g in grads:
+        for leaf in leaves[:2]:
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad(y.sum() + g.square().sum(), leaf, retain_graph=True)
+    y.square().sum().backward()
+    assert all(t.grad is not None for t in leaves)
