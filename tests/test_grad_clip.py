@@ -168,3 +168,46 @@ def test_refusals(device):
     if device == "cuda":
         with pytest.raises(ValueError):
             grad_norm([g[0], torch.ones(3)])
+
+
+# far from 1: squares past the ends of fp32's range, and one value far above the others
+SCALES = [(F32, 1e25), (BF, 1e25), (F32, 1e-25), (BF, 1e-25), (F32, 1e-21), (BF, 1e-21), (F32, 1e-38)]
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("dtype,scale", SCALES)
+def test_norms_of_very_large_and_small_gradients(dtype, scale, device):
+    from graspo_b200.ops.grad_clip import clip_grad_norm_, grad_norm
+
+    for sizes, flat in (([1], False), ([5, 12291, 70001, 3, 1000003], True), ([4096, 17], False)):
+        grads = [(g.float() * scale).to(dtype) for g in _grads(sizes, [F32], device, flat=flat)]
+        want = _norm64(grads)
+        assert want > 0
+        small = 2.0 ** -149                        # a norm below fp32's normal range is stored with fewer bits
+        assert abs(float(grad_norm(grads)) - want) <= 24 * U * want + small
+        if scale > 1:
+            out = [torch.empty_like(g, dtype=F32) for g in grads]
+            clip_grad_norm_(grads, want / 3, out=out)
+            _check_scaled(grads, out, 1 / 3)
+        else:
+            before = [g.clone() for g in grads]
+            clip_grad_norm_(grads, 1.0)            # below the limit
+            assert all(torch.equal(a, b) for a, b in zip(grads, before))
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("big,at", [(3e19, 0), (3e19, 5000), (-2e30, 12345), (1e-30, 7)])
+def test_one_value_far_from_the_others(big, at, device):
+    """One large value among ordinary ones; a tiny one among zeros."""
+    from graspo_b200.ops.grad_clip import clip_grad_norm_, grad_norm
+
+    (g,) = _grads([20011], [F32], device)
+    if abs(big) < 1:
+        g.zero_()
+    g[at] = big
+    want = _norm64([g])
+    assert abs(float(grad_norm([g])) - want) <= 24 * U * want
+    if abs(big) > 1:
+        out = torch.empty_like(g)
+        clip_grad_norm_([g], want / 4, out=[out])
+        _check_scaled([g], [out], 0.25)
