@@ -23,8 +23,8 @@
 // Rows that are no multiple of 16 bytes are read value by value; rows past the
 // variants below are walked several times (they stay in L1/L2).
 //
-// Measured on a B200, 65536 x 1152 bf16: forward 47 us (6.4 TB/s), backward 103 us
-// (4.4 TB/s; 150 us with the rows in registers), 5003 x 1001 fp32 20 and 20 us.
+// Measured on a B200, 65536 x 1152 bf16: forward 47 us (6.4 TB/s), backward 107 us
+// (4.2 TB/s; 150 us with the rows in registers), 5003 x 1001 fp32 20 and 20 us.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -546,7 +546,11 @@ __global__ void __maxnreg__(V * VPT * R <= 16 ? 104 : 128) ln_bwd_kernel(const N
 // The register form kept 9 warps of 104 registers on an SM, whose loads in flight
 // reached 2.9 TB/s; the ring holds some 100 KB of loads whatever the registers do.
 // A stage is read before its rows' barrier and refilled after it by one thread, so
-// it needs no second barrier.  4 values per thread and row.
+// it needs no second barrier.  4 values per thread and row.  Where a wait gives up,
+// that barrier tells the whole block, which fills no stage again and ends there; the
+// copies under way are waited for, whatever the error word says, since the next
+// block on the SM gets this one's shared memory.  (Through shared memory: 103 -> 107 us; a
+// barrier with a vote, or leaving the loop, made the kernel spill, 187 us.)
 constexpr int kRing = 3;
 
 template <typename T, int R>
@@ -554,6 +558,7 @@ __global__ void __maxnreg__(80) ln_bwd_ring_kernel(const NormArgs a) {
   constexpr int V = 4;
   extern __shared__ __align__(128) uint8_t ring[];   // [stage][x, dy][row][H]
   __shared__ __align__(8) uint64_t full[kRing];
+  __shared__ int late[2];                  // [turn] whether a wait gave up
   __shared__ float part_s[2][2 * R][17];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const bool mine_in = static_cast<int>(threadIdx.x) * V < a.H;
@@ -561,7 +566,8 @@ __global__ void __maxnreg__(80) ln_bwd_ring_kernel(const NormArgs a) {
   const uint32_t row_bytes = a.H * sizeof(T);
   const uint32_t stage_bytes = 2 * R * row_bytes;
   const long per = (a.rows + gridDim.x - 1) / gridDim.x;
-  const long begin = min(a.rows, blockIdx.x * per), end = min(a.rows, begin + per);
+  const long begin = min(a.rows, blockIdx.x * per);
+  long end = min(a.rows, begin + per);
   const auto fill = [&](long r0, int stage) {   // one thread
     if (r0 >= end) return;
     const int rows = static_cast<int>(min(static_cast<long>(R), end - r0));
@@ -574,6 +580,7 @@ __global__ void __maxnreg__(80) ln_bwd_ring_kernel(const NormArgs a) {
   };
   if (threadIdx.x == 0) {
     for (int s = 0; s < kRing; ++s) mbar_init(&full[s], 1);
+    late[0] = late[1] = 0;
     fence_mbar_init();
     for (int s = 0; s < kRing; ++s) fill(begin + s * R, s);
   }
@@ -600,7 +607,7 @@ __global__ void __maxnreg__(80) ln_bwd_ring_kernel(const NormArgs a) {
   int turn = 0, stage = 0;
   uint32_t phase = 0;
   for (long r0 = begin; r0 < end; r0 += R) {
-    mbar_wait(&full[stage], phase, a.err, kErrTmaFullTimeout);   // late rows leave the error word set
+    if (!mbar_wait(&full[stage], phase, a.err, kErrTmaFullTimeout)) late[turn] = 1;
     Two n[R][2], gw[R][2];
     float s[2 * R], scale[R];
     const T* at = reinterpret_cast<const T*>(ring + stage * stage_bytes) + threadIdx.x * V;
@@ -633,6 +640,7 @@ __global__ void __maxnreg__(80) ln_bwd_ring_kernel(const NormArgs a) {
     constexpr int kSpread = 32 / (2 * R);
     if (lane % kSpread == 0) part_s[turn][lane / kSpread][warp] = mine;
     __syncthreads();
+    if (late[turn] != 0) end = r0;
     if (threadIdx.x == 0) fill(r0 + kRing * R, stage);  // everyone has read this stage
     if (++stage == kRing) {
       stage = 0;
@@ -654,6 +662,11 @@ __global__ void __maxnreg__(80) ln_bwd_ring_kernel(const NormArgs a) {
       if (mine_in && r0 + j < end) store_pack<T, V>(dx, o);
     }
   }
+  if (threadIdx.x == 0)   // what was filled and not read
+    for (long r0 = end; r0 < min(min(a.rows, begin + per), end + kRing * R); r0 += R) {
+      const long i = (r0 - begin) / R;
+      mbar_wait(&full[i % kRing], static_cast<uint32_t>(i / kRing) & 1u, nullptr, kErrTmaFullTimeout);
+    }
   if (mine_in) {
     float* part = a.part + static_cast<long>(blockIdx.x) * 2 * a.H + threadIdx.x * V;
 #pragma unroll

@@ -279,3 +279,23 @@ def test_second_derivatives_are_refused(device):
                 torch.autograd.grad(y.sum() + g.square().sum(), leaf, retain_graph=True)
     y.square().sum().backward()
     assert all(t.grad is not None for t in leaves)
+
+
+@pytest.mark.gpu
+def test_waits_that_give_up_end_the_call():
+    """With an error already recorded a wait may give up: the call ends, the error is raised, the next call is right."""
+    from graspo_b200.ops._ext import KernelTimeout, check_errors, err_word
+    from graspo_b200.ops.layer_norm import layer_norm_backward, layer_norm_forward
+
+    x, w, b, dy = _case(20000, 1152, torch.bfloat16)
+    _, mean, rstd = layer_norm_forward(x, w, b)
+    want = layer_norm_backward(dy, x, w, mean, rstd)
+    check_errors()
+    for _ in range(3):
+        err_word(x.device)[0] = 1
+        layer_norm_backward(dy, x, w, mean, rstd)
+        with pytest.raises(KernelTimeout):
+            check_errors()
+        got = layer_norm_backward(dy, x, w, mean, rstd)
+        check_errors()
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
