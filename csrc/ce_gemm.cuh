@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* done = tempty + 2;   // every product issued has ended
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -196,6 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], kEpilogue);
     }
+    mbar_init(done, 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
@@ -251,9 +253,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // no copy into this CTA's shared memory may be in flight at its exit
+      // No copy into this CTA's shared memory may be in flight at its exit, after a wait
+      // that gave up either: the last fill of every stage is waited for, whatever the
+      // error word says (a stage never filled counts as complete).
       for (int s = 0; s < STAGES; ++s) {
-        if (!mbar_wait(&empty[stage], phase ^ 1u, args.err, kErrSmemEmptyTimeout)) break;
+        mbar_wait(&full[stage], phase ^ 1u, nullptr, kErrTmaFullTimeout);
         if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
@@ -302,6 +306,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++acc_iter;
         }
       }
+      // nor any product, whose accumulators are given back below
+      umma_commit(done);
+      mbar_wait(done, 0, nullptr, kErrTmemFullTimeout);
     }
   } else {
     // ------------------------------------------------------------ epilogue

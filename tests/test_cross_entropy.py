@@ -443,3 +443,22 @@ def test_second_derivatives_of_the_cpu_form():
         both.append(torch.autograd.grad(da.square().sum() + db.square().sum(), (a, b)))
     for x, y in zip(*both):                                  # fp32 sums of at most 11 terms of order 1
         assert (x - y).abs().max() < 64 * 2.0 ** -23
+
+
+@pytest.mark.gpu
+def test_waits_that_give_up_end_the_call():
+    """With an error already recorded a wait may give up: the call ends, the error is raised, the next call is right."""
+    from graspo_b200.ops._ext import KernelTimeout, check_errors, err_word
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(700, 520, 9000, 0.8, seed=13)
+    want = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none", piece=2048)
+    check_errors()
+    for _ in range(3):
+        err_word(h.device)[0] = 1
+        linear_cross_entropy_grads(h, w, t, grad=up, reduction="none", piece=2048)
+        with pytest.raises(KernelTimeout):
+            check_errors()
+        got = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none", piece=2048)
+        check_errors()
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
