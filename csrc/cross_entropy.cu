@@ -48,7 +48,8 @@ constexpr int kTokens = 32;     // tokens per block of ce_compact
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
-// What the forward leaves for the backward, in one int32 tensor.
+// What the forward leaves for the backward, in one int32 tensor.  `unit` and `ratio`
+// are those of an upstream gradient of 1; a backward of its own replaces them.
 struct State {
   int* count;           // number of trained tokens
   float* unit;          // what the tokens' weights are multiples of
@@ -534,7 +535,11 @@ std::vector<torch::Tensor> ce_backward(torch::Tensor hc, torch::Tensor state, to
   auto stream = at::cuda::getCurrentCUDAStream();
   torch::Tensor dh, dW;
   if (!want_h && !want_w) return {dh, dW};
-  const State st(state, cap);
+  // two backward passes of one graph may run at once: the weights are this call's own
+  State st(state, cap);
+  torch::Tensor weights = torch::empty({4 + (reduction == kNone ? cap : 0)}, hc.options().dtype(torch::kFloat32));
+  st.unit = weights.data_ptr<float>();
+  if (reduction == kNone) st.ratio = st.unit + 4;
   ce_weight_kernel<<<1, 1024, 0, stream>>>(g, reduction == kNone, reduction == kMean, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (want_h) dh = torch::empty({tokens, H}, hc.options());

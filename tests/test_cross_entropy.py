@@ -462,3 +462,24 @@ def test_waits_that_give_up_end_the_call():
         got = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none", piece=2048)
         check_errors()
         assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_backward_leaves_the_saved_state_alone():
+    """Two backward passes of one graph, on two streams too, each have their own weights."""
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy
+
+    h, w, t, up = _case(300, 128, 999, 0.8, seed=12)
+    hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    for reduction, first, second in (("none", up, 3 * up.flip(0)), ("mean", torch.tensor(0.3, device="cuda"),
+                                                                     torch.tensor(-7.0, device="cuda"))):
+        loss = linear_cross_entropy(hl, wl, t, reduction=reduction)
+        saved = [s.clone() for s in loss.grad_fn.saved_tensors]
+        one = torch.autograd.grad(loss, (hl, wl), first, retain_graph=True)
+        two = torch.autograd.grad(loss, (hl, wl), second, retain_graph=True)
+        # bits: rows that no token filled hold anything, NaN among it
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+                   for a, b in zip(saved, loss.grad_fn.saved_tensors))
+        again = torch.autograd.grad(loss, (hl, wl), first)
+        assert all(torch.equal(a, b) for a, b in zip(one, again))
+        assert not torch.equal(one[0], two[0])
