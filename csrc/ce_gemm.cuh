@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_col = static_cast<uint32_t>(half * 128) + (static_cast<uint32_t>(quarter * 32) << 16);
     const int align = (args.ldc & 15) == 0 ? 32 : (args.ldc & 7) == 0 ? 16 : 2;
     constexpr float kLog2e = 1.4426950408889634f;
-    const float unit = MODE == kDw ? __ldg(args.unit) : 1.f;
+    const float unit = MODE == kDw ? __ldcg(args.unit) : 1.f;
     int acc_iter = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const Unit w = decode_unit(u, num_m, num_n, splits, kb_total);
@@ -456,11 +456,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Launches a kernel of the loss's chain.  `early`: it may start while its
 // predecessor runs; it comes up beside it and waits in pdl_wait().  Every kernel of
 // the chain calls pdl_wait() before it touches memory, in every thread, so that the
-// end of one implies the end of all before it.  Between kernels of some 8 us the
-// gaps were a fifth of the time (61 tokens x 512 x 4096: 51 us without, 40 with); at
-// 6144 x 4096 x 151936 the waiting blocks take up room that the running kernel's last
-// tiles share (25.9 ms without, 28.4 with), and at 466 x 1000 x 50001 it made no
-// difference.  kEarlyWork lies in between.
+// end of one implies the end of all before it.  What the chain writes is read by
+// plain or L2 loads, never through `const __restrict__` or __ldg: those are for
+// memory that is constant while a kernel lives, and an early one lives before it is
+// written.  Between kernels of some 8 us the gaps were a fifth of the time (61 tokens
+// x 512 x 4096: 51 us without, 40 with); at 6144 x 4096 x 151936 the waiting blocks
+// take up room that the running kernel's last tiles share (25.9 ms without, 28.4
+// with), and at 466 x 1000 x 50001 it made no difference.  kEarlyWork lies in between.
 constexpr double kEarlyWork = 4e9;   // tokens x vocabulary x hidden
 
 template <typename... KArgs, typename... A>

@@ -193,7 +193,7 @@ __device__ __forceinline__ float common_weight(const float* g, bool mean, int n)
 // of the largest logit's last place, 2e-6 at 20 and 3e-5 at 300, where a confident
 // token's loss is 1e-6.)  p - 1 = expm1(-loss) likewise: exp(l - lse) - 1 from the
 // remade logit was off by 2.5e-5, a quarter of it at a loss of 1e-4.
-__global__ void __launch_bounds__(kBlock) ce_finish_kernel(const float2* __restrict__ part, int parts, State st,
+__global__ void __launch_bounds__(kBlock) ce_finish_kernel(const float2* part, int parts, State st,
                                                              const float* __restrict__ g, bool mean,
                                                              float* __restrict__ loss) {
   pdl_trigger();
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(1024) ce_weight_kernel(const float* __restrict
 
 // Sum of the tokens' losses in a fixed order, over the trained tokens for the
 // mean (no trained token: 0).  One block.
-__device__ void total_loss(const float* __restrict__ loss, long T, int n, bool mean, float* __restrict__ out) {
+__device__ void total_loss(const float* loss, long T, int n, bool mean, float* __restrict__ out) {
   __shared__ double part[kBlock / 32];
   double s = 0;
 #pragma unroll 8
@@ -272,7 +272,7 @@ __device__ void total_loss(const float* __restrict__ loss, long T, int n, bool m
   }
 }
 
-__global__ void __launch_bounds__(kBlock) ce_total_kernel(const float* __restrict__ loss, long T, State st, bool mean,
+__global__ void __launch_bounds__(kBlock) ce_total_kernel(const float* loss, long T, State st, bool mean,
                                                             float* __restrict__ out) {
   pdl_trigger();
   pdl_wait();
@@ -282,10 +282,10 @@ __global__ void __launch_bounds__(kBlock) ce_total_kernel(const float* __restric
 // dh[t] = unit * sum of the slices' row place[t], rounded once; zero for an
 // ignored token.  A last block adds the losses up where `total` wants them.
 template <bool WIDE>
-__global__ void __launch_bounds__(kBlock) ce_scatter_kernel(const float* __restrict__ acc, int lda, State st, long T,
+__global__ void __launch_bounds__(kBlock) ce_scatter_kernel(const float* acc, int lda, State st, long T,
                                                               int H, int kb_first, int sms,
                                                               __nv_bfloat16* __restrict__ dh,
-                                                              const float* __restrict__ loss, bool mean,
+                                                              const float* loss, bool mean,
                                                               float* __restrict__ total) {
   pdl_trigger();
   pdl_wait();

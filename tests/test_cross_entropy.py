@@ -483,3 +483,24 @@ def test_backward_leaves_the_saved_state_alone():
         again = torch.autograd.grad(loss, (hl, wl), first)
         assert all(torch.equal(a, b) for a, b in zip(one, again))
         assert not torch.equal(one[0], two[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_calls_in_a_row_do_not_mix(reduction):
+    """Small calls start their kernels early: many of them back to back, each with its own unit and number of tokens,
+    give what each gives by itself."""
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    cases = []
+    for i in range(4):
+        h, w, t, up = _case(61 + 40 * i, 512, 4096, 0.9 - 0.2 * i, seed=20 + i)
+        cases.append((h, w, t, up * 10.0 ** (3 * i - 4) if reduction == "none" else up[0].abs() * 10.0 ** (3 * i - 4)))
+    want = []
+    for h, w, t, g in cases:
+        want.append(linear_cross_entropy_grads(h, w, t, grad=g, reduction=reduction))
+        torch.cuda.synchronize()
+    got = [linear_cross_entropy_grads(h, w, t, grad=g, reduction=reduction)
+           for _ in range(60) for h, w, t, g in cases]
+    for i, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i % 4]))
