@@ -832,7 +832,8 @@ torch::Tensor as_rows(const torch::Tensor& t) {
 }
 
 void check_x(const torch::Tensor& x) {
-  require(x.is_cuda() && is_storage_type(x) && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < (1L << 30),
+  // (the column sums' 2 H indexes, rounded up to blocks of 32, are ints)
+  require(x.is_cuda() && is_storage_type(x) && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= (1L << 30) - 16,
           "x must be a bf16, fp16 or fp32 CUDA tensor with a last dimension to normalise");
 }
 

@@ -299,3 +299,16 @@ def test_waits_that_give_up_end_the_call():
         got = layer_norm_backward(dy, x, w, mean, rstd)
         check_errors()
         assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_rows_too_long_for_the_column_sums_are_refused():
+    """Twice the row's length is an int in the backward: the last lengths below 2^30 are refused up front."""
+    from graspo_b200.ops.layer_norm import layer_norm_backward, layer_norm_forward
+
+    H = (1 << 30) - 15
+    one = torch.ones(1, 1, device="cuda", dtype=torch.bfloat16).expand(1, H)
+    with pytest.raises(ValueError):
+        layer_norm_forward(one, one[0], None)
+    with pytest.raises(ValueError):
+        layer_norm_backward(one, one, one[0], torch.zeros(1, device="cuda"), torch.ones(1, device="cuda"))
