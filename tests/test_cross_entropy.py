@@ -504,3 +504,53 @@ def test_calls_in_a_row_do_not_mix(reduction):
            for _ in range(60) for h, w, t, g in cases]
     for i, out in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(out, want[i % 4]))
+
+
+# Rules on sizes choose segments, launches, slices and pieces; each row reaches one that SHAPES does not.
+LARGE = [
+    # tokens, hidden, vocabulary, share of trained tokens
+    (40, 1025, 300, 1.0),           # a second segment of one K-block
+    (61, 2056, 515, 0.8),           # three segments
+    (70, 4096, 600, 1.0),           # four segments
+    (700, 136, 12000, 1.0),         # 282 tiles: a CTA takes several
+    (600, 2048, 4100, 1.0),         # kernels launched one after the other
+    (2432, 2048, 4100, 1.0),        # 152 tiles of dh, in two slices
+    (8200, 72, 16500, 0.9),         # two pieces of the vocabulary by default
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,V,valid", LARGE)
+def test_larger_shapes_against_64_bits(T, H, V, valid):
+    from graspo_b200.ops._ext import check_errors
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(T, H, V, valid, seed=T)
+    loss, dh, dw = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none")
+    check_errors()
+    want, wh, ww, bound = _oracle(h, w, t, up)
+    _within(loss, want, bound["loss"], "loss")
+    _within(dh, wh, bound["dh"], "dh")
+    _within(dw, ww, bound["dw"], "dw")
+    again = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none")
+    assert all(torch.equal(a, b) for a, b in zip((loss, dh, dw), again)), "two calls differ"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,V,valid,piece", [(61, 512, 4096, 0.8, 0), (333, 1001, 777, 0.6, 256),
+                                               (600, 2048, 4100, 0.7, 0), (1, 8, 1, 1.0, 0)])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("upstream", [None, -1.75])
+def test_reduced_loss_and_gradients_in_one_call(T, H, V, valid, piece, reduction, upstream):
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, _ = _case(T, H, V, valid, seed=T + 1)
+    grad = None if upstream is None else torch.tensor(upstream, device="cuda")
+    loss, dh, dw = linear_cross_entropy_grads(h, w, t, grad=grad, reduction=reduction, piece=piece)
+    k = 1 / int((t != IGNORE).sum()) if reduction == "mean" else 1.0
+    want, wh, ww, bound = _oracle(h, w, t, torch.full((T,), (upstream or 1.0) * k, device="cuda", dtype=torch.float64))
+    assert loss.shape == () and loss.dtype == torch.float32
+    assert abs(float(loss) - float(want.sum()) * k) <= (float(bound["loss"].sum()) * k
+                                                        + 2.0 ** -23 * float(want.sum()) * k)
+    _within(dh, wh, bound["dh"], "dh")
+    _within(dw, ww, bound["dw"], "dw")
