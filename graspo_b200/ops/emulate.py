@@ -1,4 +1,4 @@
-"""Plain-PyTorch emulation of every kernel-library entry point.
+"""Plain-PyTorch emulation of the kernel library's entry points.
 
 Same names and signatures as ``graspo_b200._C``; results are computed with
 ordinary tensor operations in fp32 and stored in the caller's buffers.  It
@@ -6,7 +6,9 @@ exists for CPU tests of the fused orchestration code (layouts, LoRA
 K-extension, split-K workspaces, paged cache bookkeeping): with
 ``use_emulation()`` active, ``ext()`` returns this module, so the fused
 model, rollout engine and optimizer run on a machine without a GPU and can be
-compared with the eager oracle.  It is never used on a GPU run.
+compared with the eager oracle.  It is never used on a GPU run.  (Operators that
+compute with PyTorch where their tensors are on the CPU -- embedding, layer norm,
+gradient clipping, the cross entropy's one-call gradients -- do not come here.)
 """
 
 from __future__ import annotations
@@ -399,7 +401,6 @@ def sample_append_split(logits, temperature, seed, next_ids, slot, pos, kv_len, 
                   eos_id, pad_id, ignore_eos, None)
 
 
-
 def _ce_live(targets, V, ignore_index):
     return (targets != ignore_index) & (targets >= 0) & (targets < V)
 
@@ -444,46 +445,3 @@ def ce_backward(hc, state, W, tokens, grad, reduction, want_h, want_w, piece, er
     dh = torch.zeros(tokens, H, dtype=hc.dtype)
     dh[rows] = (acc * unit).to(dh.dtype)
     return (dh if want_h else None), (dw if want_w else None)
-
-
-def ce_grads(h, W, targets, grad, ignore_index, reduction, want_w, piece, err):
-    loss, hc, state = ce_forward(h, W, targets, ignore_index, reduction, err)
-    up = torch.ones(targets.numel() if reduction == 0 else 1) if grad is None else grad.reshape(-1)
-    dh, dw = ce_backward(hc, state, W, targets.numel(), up, reduction, True, want_w, piece, err)
-    return loss, dh.view(h.shape), dw
-
-
-def embed_fwd(ids, table, scale, err):
-    from graspo_b200.ops.embedding import embedding
-
-    return embedding(ids, table, scale=scale)
-
-
-def embed_bwd(dy, ids, vocab, into, scale, padding, err):
-    from graspo_b200.ops.embedding import embedding_grad
-
-    return embedding_grad(dy, ids, vocab, scale=scale, padding_idx=None if padding < 0 else padding, out=into)
-
-
-def layer_norm_fwd(x, w, b, eps):
-    from graspo_b200.ops.layer_norm import layer_norm_forward
-
-    return layer_norm_forward(x, w, b, eps)
-
-
-def layer_norm_bwd(dy, x, w, mean, rstd, bias32, err):
-    from graspo_b200.ops.layer_norm import layer_norm_backward
-
-    return layer_norm_backward(dy, x, w, mean, rstd, torch.float32 if bias32 else x.dtype)
-
-
-def grad_norm(grads, device):
-    from graspo_b200.ops.grad_clip import grad_norm as norm
-
-    return norm(grads)
-
-
-def grad_clip(grads, out, max_norm, device):
-    from graspo_b200.ops.grad_clip import clip_grad_norm_
-
-    return clip_grad_norm_(grads, max_norm, out=out or None)
