@@ -96,14 +96,13 @@ void adamw(torch::Tensor p, torch::Tensor g, torch::Tensor m, torch::Tensor v, d
            double b2, double eps, double wd, int64_t step, torch::Tensor sumsq, double max_norm,
            c10::optional<torch::Tensor> loss, c10::optional<torch::Tensor> skipped);
 void transpose_bf16(torch::Tensor in, torch::Tensor out);
-std::vector<torch::Tensor> ce_forward(torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index,
-                                      int64_t reduction, torch::Tensor err);
-std::vector<torch::Tensor> ce_backward(torch::Tensor hc, torch::Tensor state, torch::Tensor W, int64_t tokens,
-                                       torch::Tensor grad, int64_t reduction, bool want_h, bool want_w, int64_t piece,
-                                       torch::Tensor err);
-std::vector<torch::Tensor> ce_grads(torch::Tensor h, torch::Tensor W, torch::Tensor targets,
-                                    c10::optional<torch::Tensor> grad, int64_t ignore_index, int64_t reduction,
-                                    bool want_w, int64_t piece, torch::Tensor err);
+using Launched = std::pair<std::vector<torch::Tensor>, int64_t>;
+Launched ce_forward(torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index, int64_t reduction,
+                    torch::Tensor err);
+Launched ce_backward(torch::Tensor hc, torch::Tensor state, torch::Tensor W, int64_t tokens, torch::Tensor grad,
+                     int64_t reduction, bool want_h, bool want_w, int64_t piece, torch::Tensor err);
+Launched ce_grads(torch::Tensor h, torch::Tensor W, torch::Tensor targets, c10::optional<torch::Tensor> grad,
+                  int64_t ignore_index, int64_t reduction, bool want_w, int64_t piece, torch::Tensor err);
 torch::Tensor embed_fwd(torch::Tensor ids, torch::Tensor table, double scale, torch::Tensor err);
 torch::Tensor embed_bwd(torch::Tensor dy, torch::Tensor ids, int64_t vocab, c10::optional<torch::Tensor> into,
                         double scale, int64_t padding, torch::Tensor err);
@@ -207,12 +206,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw", &gb::adamw);
   m.def("transpose_bf16", &gb::transpose_bf16);
   m.def("ce_forward", &gb::ce_forward,
-        "cross entropy over a vocabulary projection: the loss and the state of its backward", py::arg("h"),
+        "cross entropy over a vocabulary projection: (loss and the state of its backward), launches", py::arg("h"),
         py::arg("W"), py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"), py::arg("err"));
-  m.def("ce_backward", &gb::ce_backward, "gradients of the cross entropy, in pieces of the vocabulary", py::arg("hc"),
+  m.def("ce_backward", &gb::ce_backward, "(gradients of the cross entropy, in pieces of the vocabulary), launches", py::arg("hc"),
         py::arg("state"), py::arg("W"), py::arg("tokens"), py::arg("grad"), py::arg("reduction"), py::arg("want_h"),
         py::arg("want_w"), py::arg("piece"), py::arg("err"));
-  m.def("ce_grads", &gb::ce_grads, "the cross entropy and its gradients in one call", py::arg("h"), py::arg("W"),
+  m.def("ce_grads", &gb::ce_grads, "(the cross entropy and its gradients), launches", py::arg("h"), py::arg("W"),
         py::arg("targets"), py::arg("grad"), py::arg("ignore_index"), py::arg("reduction"), py::arg("want_w"),
         py::arg("piece"), py::arg("err"));
   m.def("embed_fwd", &gb::embed_fwd, "scaled embedding lookup", py::arg("ids"), py::arg("table"), py::arg("scale"),

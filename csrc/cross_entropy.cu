@@ -362,6 +362,7 @@ bool launches_early(int64_t cap, int64_t V, int64_t H) {
 struct Forward {
   torch::Tensor loss, hc, state, W;   // loss per token; W as TMA reads it
   int64_t T, H, V, cap, Hp;
+  int64_t launches;
 };
 
 Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Tensor& targets, int64_t ignore_index,
@@ -401,11 +402,13 @@ Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Ten
   ce::launch_chained(args.early, ce_finish_kernel, static_cast<unsigned>(std::min<int64_t>((f.cap + 7) / 8, 148 * 8)), kBlock, 0,
                      stream, static_cast<const float2*>(args.part), 2 * num_n, st, grad, reduction == kMean,
                      f.loss.data_ptr<float>());
+  f.launches = 3 + !f.W.is_same(W);
   return f;
 }
 
-// dh [T, H] with the loss's total (where `total` is given), and dW [V, H].
-void backward(const torch::Tensor& hc, const State& st, const torch::Tensor& W, int64_t T, int64_t V, int64_t H,
+// dh [T, H] with the loss's total (where `total` is given), and dW [V, H].  The
+// number of kernels launched.
+int64_t backward(const torch::Tensor& hc, const State& st, const torch::Tensor& W, int64_t T, int64_t V, int64_t H,
               int64_t piece, torch::Tensor* dh, torch::Tensor* dW, const torch::Tensor& loss, bool mean,
               torch::Tensor* total, int* err, cudaStream_t stream) {
   const int device = hc.get_device();
@@ -474,6 +477,8 @@ void backward(const torch::Tensor& hc, const State& st, const torch::Tensor& W, 
                        static_cast<const float*>(loss.defined() ? loss.data_ptr<float>() : nullptr), mean,
                        total != nullptr ? total->data_ptr<float>() : nullptr);
   }
+  const int64_t pieces = (V + piece - 1) / piece, each = 1 + (dh != nullptr) + (dW != nullptr);
+  return pieces * each + (dh != nullptr);
 }
 
 void check_inputs(const torch::Tensor& h, const torch::Tensor& W, const torch::Tensor& targets, int64_t reduction) {
@@ -506,26 +511,28 @@ torch::Tensor flat_targets(const torch::Tensor& t) {
 
 }  // namespace
 
+// Each with the number of kernels launched.
+using Launched = std::pair<std::vector<torch::Tensor>, int64_t>;
+
 // (loss, compacted h, state): what ce_backward needs.
-std::vector<torch::Tensor> ce_forward(torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index,
+Launched ce_forward(torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index,
                                       int64_t reduction, torch::Tensor err) {
   check_inputs(h, W, targets, reduction);
   const c10::cuda::CUDAGuard guard(h.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   const Forward f = forward(h, W, flat_targets(targets), ignore_index, nullptr, reduction, err.data_ptr<int>(), stream);
-  if (reduction == kNone) return {f.loss.view(targets.sizes()), f.hc, f.state};
+  if (reduction == kNone) return {{f.loss.view(targets.sizes()), f.hc, f.state}, f.launches};
   torch::Tensor total = torch::empty({}, f.loss.options());
   ce_total_kernel<<<1, kBlock, 0, stream>>>(f.loss.data_ptr<float>(), f.T, State(f.state, f.cap), reduction == kMean,
                                               total.data_ptr<float>());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {total, f.hc, f.state};
+  return {{total, f.hc, f.state}, f.launches + 1};
 }
 
 // (dh [tokens, H], dW); what is not wanted is None.  grad: fp32, one value, or one
 // per token for reduction none.
-std::vector<torch::Tensor> ce_backward(torch::Tensor hc, torch::Tensor state, torch::Tensor W, int64_t tokens,
-                                       torch::Tensor grad, int64_t reduction, bool want_h, bool want_w, int64_t piece,
-                                       torch::Tensor err) {
+Launched ce_backward(torch::Tensor hc, torch::Tensor state, torch::Tensor W, int64_t tokens, torch::Tensor grad,
+                     int64_t reduction, bool want_h, bool want_w, int64_t piece, torch::Tensor err) {
   const int64_t H = W.size(1), V = W.size(0), cap = capacity(tokens);
   require(hc.is_cuda() && hc.size(0) == cap && hc.size(1) == round_up(H, kColumnPad) && state.numel() == State::words(cap),
           "state of another call");
@@ -534,7 +541,7 @@ std::vector<torch::Tensor> ce_backward(torch::Tensor hc, torch::Tensor state, to
   const c10::cuda::CUDAGuard guard(hc.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   torch::Tensor dh, dW;
-  if (!want_h && !want_w) return {dh, dW};
+  if (!want_h && !want_w) return {{dh, dW}, 0};
   // two backward passes of one graph may run at once: the weights are this call's own
   State st(state, cap);
   torch::Tensor weights = torch::empty({4 + (reduction == kNone ? cap : 0)}, hc.options().dtype(torch::kFloat32));
@@ -544,15 +551,15 @@ std::vector<torch::Tensor> ce_backward(torch::Tensor hc, torch::Tensor state, to
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (want_h) dh = torch::empty({tokens, H}, hc.options());
   if (want_w) dW = torch::empty({V, H}, hc.options());
-  backward(hc, st, tma_rows(W, tokens, stream), tokens, V, H, piece, want_h ? &dh : nullptr, want_w ? &dW : nullptr,
-           torch::Tensor(), false, nullptr, err.data_ptr<int>(), stream);
-  return {dh, dW};
+  const torch::Tensor Wt = tma_rows(W, tokens, stream);
+  const int64_t n = backward(hc, st, Wt, tokens, V, H, piece, want_h ? &dh : nullptr, want_w ? &dW : nullptr,
+                             torch::Tensor(), false, nullptr, err.data_ptr<int>(), stream);
+  return {{dh, dW}, 1 + !Wt.is_same(W) + n};
 }
 
 // (loss, dh, dW) in one call; dW is None where it is not wanted.
-std::vector<torch::Tensor> ce_grads(torch::Tensor h, torch::Tensor W, torch::Tensor targets,
-                                    c10::optional<torch::Tensor> grad, int64_t ignore_index, int64_t reduction,
-                                    bool want_w, int64_t piece, torch::Tensor err) {
+Launched ce_grads(torch::Tensor h, torch::Tensor W, torch::Tensor targets, c10::optional<torch::Tensor> grad,
+                  int64_t ignore_index, int64_t reduction, bool want_w, int64_t piece, torch::Tensor err) {
   check_inputs(h, W, targets, reduction);
   check_piece(piece);
   const float* g = check_grad(grad, h, reduction, targets.numel());
@@ -562,15 +569,16 @@ std::vector<torch::Tensor> ce_grads(torch::Tensor h, torch::Tensor W, torch::Ten
   const Forward f = forward(h, W, flat_targets(targets), ignore_index, reduction == kNone ? nullptr : g, reduction, e,
                             stream);
   const State st(f.state, f.cap);
-  if (reduction == kNone && g != nullptr) {
+  const bool weighted = reduction == kNone && g != nullptr;
+  if (weighted) {
     ce::launch_chained(launches_early(f.cap, f.V, f.H), ce_weight_kernel, 1, 1024, 0, stream, g, true, false, st);
   }
   torch::Tensor dh = torch::empty(h.sizes(), h.options()), dW, total;
   if (want_w) dW = torch::empty({f.V, f.H}, h.options());
   if (reduction != kNone) total = torch::empty({}, f.loss.options());
-  backward(f.hc, st, f.W, f.T, f.V, f.H, piece, &dh, want_w ? &dW : nullptr, f.loss, reduction == kMean,
-           reduction != kNone ? &total : nullptr, e, stream);
-  return {reduction == kNone ? f.loss.view(targets.sizes()) : total, dh, dW};
+  const int64_t n = backward(f.hc, st, f.W, f.T, f.V, f.H, piece, &dh, want_w ? &dW : nullptr, f.loss,
+                             reduction == kMean, reduction != kNone ? &total : nullptr, e, stream);
+  return {{reduction == kNone ? f.loss.view(targets.sizes()) : total, dh, dW}, f.launches + weighted + n};
 }
 
 }  // namespace gb

@@ -67,8 +67,9 @@ def _torch_loss(h, weight, targets, ignore_index, reduction):
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, weight, targets, ignore_index, reduction, piece, h_edge=None):
-        launches.add(2 + (reduction != "none"))      # compaction, product, row sums (and their total)
-        loss, *state = ext().ce_forward(h, weight, targets, ignore_index, REDUCTIONS[reduction], err_word(h.device))
+        (loss, *state), count = ext().ce_forward(h, weight, targets, ignore_index, REDUCTIONS[reduction],
+                                                 err_word(h.device))
+        launches.add(count - 1)
         ctx.save_for_backward(weight, h_edge, *state)
         ctx.shape, ctx.tokens, ctx.reduction, ctx.piece = h.shape, targets.numel(), reduction, piece
         return loss
@@ -76,10 +77,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         weight, h_edge, hc, state = ctx.saved_tensors
-        launches.add(4)                              # weights, three products a piece, the rows of dh
-        dh, dw = ext().ce_backward(hc, state, weight, ctx.tokens, g.float().contiguous().view(-1),
-                                   REDUCTIONS[ctx.reduction], ctx.needs_input_grad[0], ctx.needs_input_grad[1],
-                                   ctx.piece, err_word(hc.device))
+        (dh, dw), count = ext().ce_backward(hc, state, weight, ctx.tokens, g.float().contiguous().view(-1),
+                                            REDUCTIONS[ctx.reduction], ctx.needs_input_grad[0],
+                                            ctx.needs_input_grad[1], ctx.piece, err_word(hc.device))
+        launches.add(count - 1)
         dh, dw = refuse_second("linear_cross_entropy", (None if dh is None else dh.view(ctx.shape), dw),
                                g, weight, h_edge)
         return dh, dw, None, None, None, None, None
@@ -113,9 +114,9 @@ def linear_cross_entropy_grads(
     if h.is_cuda and reduction in REDUCTIONS:
         if grad is not None:
             grad = grad.detach().float().contiguous()
-        launches.add(6 + (reduction == "none" and grad is not None))    # as the two halves, one call
-        loss, dh, dw = ext().ce_grads(h, weight, targets, grad, ignore_index, REDUCTIONS[reduction], weight_grad,
-                                      piece, err_word(h.device))
+        (loss, dh, dw), count = ext().ce_grads(h, weight, targets, grad, ignore_index, REDUCTIONS[reduction],
+                                               weight_grad, piece, err_word(h.device))
+        launches.add(count - 1)
         return loss, dh, dw
     _check(h, weight, targets, reduction, piece)
     if grad is not None and (grad.numel() != (targets.numel() if reduction == "none" else 1)

@@ -423,8 +423,8 @@ def ce_forward(h, W, targets, ignore_index, reduction, err):
     loss[rows] = torch.logaddexp(torch.zeros(()), torch.logsumexp(lead, -1))
     state = torch.stack([rows.double(), t[rows].double(), lse.double(), torch.expm1(-loss[rows]).double()])
     if reduction == 0:
-        return loss.view(targets.shape), hc, state
-    return loss.sum() / (max(1, rows.numel()) if reduction == 2 else 1), hc, state
+        return (loss.view(targets.shape), hc, state), 1
+    return (loss.sum() / (max(1, rows.numel()) if reduction == 2 else 1), hc, state), 1
 
 
 def ce_backward(hc, state, W, tokens, grad, reduction, want_h, want_w, piece, err):
@@ -444,4 +444,4 @@ def ce_backward(hc, state, W, tokens, grad, reduction, want_h, want_w, piece, er
         dw[v0 : v0 + Wv.shape[0]] = (d.T @ h * unit).to(dw.dtype)
     dh = torch.zeros(tokens, H, dtype=hc.dtype)
     dh[rows] = (acc * unit).to(dh.dtype)
-    return (dh if want_h else None), (dw if want_w else None)
+    return (dh if want_h else None, dw if want_w else None), 1

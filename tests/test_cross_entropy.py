@@ -554,3 +554,28 @@ def test_reduced_loss_and_gradients_in_one_call(T, H, V, valid, piece, reduction
                                                         + 2.0 ** -23 * float(want.sum()) * k)
     _within(dh, wh, bound["dh"], "dh")
     _within(dw, ww, bound["dw"], "dw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,piece,copies,pieces", [(64, 0, 0, 1), (64, 256, 0, 4), (1001, 0, 1, 1), (1001, 512, 1, 2)])
+def test_every_launch_is_counted(H, piece, copies, pieces):
+    from graspo_b200.ops._ext import launches
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy, linear_cross_entropy_grads
+
+    h, w, t, up = _case(600, H, 1000, 0.8, seed=14)
+
+    def counted(call):
+        before = launches.count
+        out = call()
+        return launches.count - before, out
+
+    # compaction, (a copy of W's odd rows), product, row sums; per piece of the vocabulary the products; the rows of dh
+    forward = 3 + copies
+    assert counted(lambda: linear_cross_entropy_grads(h, w, t, piece=piece))[0] == forward + 3 * pieces + 1
+    assert counted(lambda: linear_cross_entropy_grads(h, w, t, piece=piece, weight_grad=False))[0] == forward + 2 * pieces + 1
+    assert counted(lambda: linear_cross_entropy_grads(h, w, t, grad=up, reduction="none", piece=piece))[0] == (
+        forward + 1 + 3 * pieces + 1)
+    hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    n, loss = counted(lambda: linear_cross_entropy(hl, wl, t, piece=piece))
+    assert n == forward + 1                                   # and the total
+    assert counted(loss.backward)[0] == 1 + copies + 3 * pieces + 1
