@@ -459,10 +459,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 // end of one implies the end of all before it.  What the chain writes is read by
 // plain or L2 loads, never through `const __restrict__` or __ldg: those are for
 // memory that is constant while a kernel lives, and an early one lives before it is
-// written.  Between kernels of some 8 us the gaps were a fifth of the time (61 tokens
-// x 512 x 4096: 51 us without, 40 with); at 6144 x 4096 x 151936 the waiting blocks
-// take up room that the running kernel's last tiles share (25.9 ms without, 28.4
-// with), and at 466 x 1000 x 50001 it made no difference.  kEarlyWork lies in between.
+// written.  Between kernels of some 8 us the gaps were a fifth of the time: without /
+// with early launches 61 x 512 x 4096 (work 1.3e8) 52 / 43 us, 512 x 1024 x 4096 (2e9)
+// 64 / 52, 1024 x 1024 x 16384 (1.7e10) 150 / 140, 128 x 2048 x 151936 (4e10) 552 / 548,
+// 1024 x 2048 x 32000 (7e10) 444 / 443; at 6144 x 4096 x 151936 (3.8e12) the waiting
+// blocks take up room that the running kernel's last tiles share (25.9 / 28.4 ms).
+// kEarlyWork keeps to calls that are certain to gain; some up to 2e10 would too.
 constexpr double kEarlyWork = 4e9;   // tokens x vocabulary x hidden
 
 template <typename... KArgs, typename... A>

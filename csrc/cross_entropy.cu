@@ -123,12 +123,13 @@ __device__ __forceinline__ void copy_row(const __nv_bfloat16* in, int H, __nv_bf
 }
 
 // The trained tokens' rows of h, one after the other, and their places.  A block
-// counts the trained tokens before its own 32 itself: 8 bytes a token from L2
-// against some 10 ns of products, and no second pass.  The last block knows the
-// count and zeroes the rows that fill the last K-block of dW (what the rest of the
-// last tile holds stays in its own rows).  A target outside the
-// vocabulary that is not ignore_index is reported in err[1] and gets a NaN loss
-// and a zero gradient.
+// counts the trained tokens before its own 32 itself, so that there is no second
+// pass.  That is T / 8 bytes a token from L2 and grows with the square of the
+// tokens: 7 us of 156 at 8192 tokens x 256 x 4096, 141 us of 4.3 ms at 131072, 6.8 of
+// 112 ms at a million.  The last block knows the count and zeroes the rows that fill
+// the last K-block of dW (what the rest of the last tile holds stays in its own
+// rows).  A target outside the vocabulary that is not ignore_index is reported in
+// err[1] and gets a NaN loss and a zero gradient.
 template <bool WIDE>
 __global__ void __launch_bounds__(kBlock) ce_compact_kernel(const int64_t* __restrict__ targets, long T, long V,
                                                               long ignore, const __nv_bfloat16* __restrict__ h, long ldh,
@@ -329,8 +330,12 @@ T* ptr(const torch::Tensor& t) {
 
 // W as TMA reads it: rows of 16-byte multiples from a 16-byte boundary.  Rows that
 // are no multiple of 32 bytes apart cross one more sector each, which every one of
-// the products that read W pays (65 against 48 us at 466 tokens x 50001 x 1000);
-// from kCopyTokens tokens on the copy costs less.
+// the products that read W pays (65 against 48 us at 466 tokens x 50001 x 1000).  Both
+// the copy and what it saves grow with V H, the latter with the tokens too; loss and
+// gradients as W is / with a copy, at 1000 x 50001, 4088 x 20001, 520 x 150001 and
+// 2056 x 151936: 256 tokens 175 / 192, 287 / 309, 294 / 330, 885 / 950 us; 512 tokens
+// 265 / 263, 417 / 419, 495 / 507, 1551 / 1509; 1024 tokens 469 / 431, 735 / 653,
+// 931 / 898, 2832 / 2530.
 constexpr int64_t kCopyTokens = 512;
 
 torch::Tensor tma_rows(const torch::Tensor& W, int64_t tokens, cudaStream_t stream) {
@@ -415,7 +420,9 @@ int64_t backward(const torch::Tensor& hc, const State& st, const torch::Tensor& 
   const int64_t cap = hc.size(0), Hp = hc.size(1);
   const bool early = launches_early(cap, V, H);
   // A piece of d is at most 256 MiB: large enough that the three products of a
-  // piece run for many waves of tiles, small against the logits.
+  // piece run for many waves of tiles, small against the logits.  256 columns are the
+  // least, which are more than that from 524289 tokens on (512 bytes a token); dW then
+  // has as few tiles as ceil(H / 256) x 2 a piece, and a call should be split.
   if (piece == 0) piece = std::max<int64_t>((256LL << 20) / (cap * 2) / ce::BN * ce::BN, ce::BN);
   piece = std::min(piece, round_up(V, ce::BN));
   torch::Tensor d = torch::empty({cap, piece}, hc.options());

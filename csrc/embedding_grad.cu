@@ -14,7 +14,9 @@
 //    shared memory across); a token's place in the whole is its place in its own
 //    chunk plus the number of smaller ids in every other chunk (a binary search
 //    each, the chunks shared out over a block's warps).  Two launches and no
-//    counters, for any number of tokens.
+//    counters, for any number of tokens; the searches grow with the square of the
+//    tokens (5 us of 32 at 8192, 104 of 180 at 131072, 5.7 of 6.0 ms at a million,
+//    each 256 columns wide).
 //  * Long runs (one id over thousands of tokens, as padding makes them): aligned
 //    groups of 32 equal tokens, and of 32 such groups, are added first, all at
 //    once, and a run then adds those sums: at most 62 tokens, 62 groups and its

@@ -95,7 +95,8 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     """Cross entropy of ``h @ weight^T`` against ``targets`` (fp32), differentiable in ``h`` and ``weight``.
 
     ``piece``: vocabulary columns per piece of the backward (a multiple of 256;
-    0 takes as many as 256 MiB of softmax gradients hold)."""
+    0 takes as many as 256 MiB of softmax gradients hold, at least 256: 512 bytes a
+    token, so split calls of more than half a million tokens)."""
     if h.is_cuda and reduction in REDUCTIONS:
         return _kernel_loss(h, weight, targets, int(ignore_index), reduction, int(piece))
     _check(h, weight, targets, reduction, piece)
