@@ -66,7 +66,8 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float,
     """Scale ``grads`` to a global norm of at most ``max_norm``; the norm before it.
 
     With ``out`` (one tensor per gradient, of its size and any of the three
-    types) the scaled values go there and ``grads`` stay as they are."""
+    types) the scaled values go there and ``grads`` stay as they are.  What is
+    written must not overlap: a tensor that is there twice is a race."""
     grads = _list(grads)
     out = None if out is None else _list(out)
     if not max_norm >= 0:
