@@ -1,4 +1,5 @@
 // Python bindings of the sm_100a kernel library (module graspo_b200._C).
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <stdexcept>
@@ -114,6 +115,23 @@ torch::Tensor grad_norm(const TensorRefs& grads, int64_t device);
 torch::Tensor grad_clip(const TensorRefs& grads, const TensorRefs& out, double max_norm, int64_t device);
 }  // namespace gb
 
+// An empty tensor with t's place in the graph, for a backward that needs t itself no
+// more (none where t requires no gradient).  A node in Python cost 11 us a call.
+namespace {
+struct EdgeNode final : torch::autograd::Node {
+  torch::autograd::variable_list apply(torch::autograd::variable_list&&) override { return {torch::Tensor()}; }
+};
+
+torch::Tensor edge_of(const torch::Tensor& t) {
+  if (!t.requires_grad()) return torch::Tensor();
+  const std::shared_ptr<torch::autograd::Node> node(new EdgeNode, torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(t));
+  torch::Tensor edge = torch::empty({0}, t.options().requires_grad(false));
+  torch::autograd::set_history(edge, node);
+  return edge;
+}
+}  // namespace
+
 // The tensors of a Python list, which holds them during the call.
 static gb::TensorRefs tensor_refs(const py::list& list) {
   gb::TensorRefs refs;
@@ -205,9 +223,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grad_sumsq", &gb::grad_sumsq);
   m.def("adamw", &gb::adamw);
   m.def("transpose_bf16", &gb::transpose_bf16);
-  m.def("ce_forward", &gb::ce_forward,
-        "cross entropy over a vocabulary projection: (loss and the state of its backward), launches", py::arg("h"),
-        py::arg("W"), py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"), py::arg("err"));
+  m.def("ce_forward",
+        [](torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index, int64_t reduction,
+           torch::Tensor err) {
+          gb::Launched r = gb::ce_forward(h, W, targets, ignore_index, reduction, err);
+          r.first.push_back(edge_of(h));
+          return r;
+        },
+        "cross entropy over a vocabulary projection: (loss, state of its backward, the place of h in the graph), launches",
+        py::arg("h"), py::arg("W"), py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"), py::arg("err"));
   m.def("ce_backward", &gb::ce_backward, "(gradients of the cross entropy, in pieces of the vocabulary), launches", py::arg("hc"),
         py::arg("state"), py::arg("W"), py::arg("tokens"), py::arg("grad"), py::arg("reduction"), py::arg("want_h"),
         py::arg("want_w"), py::arg("piece"), py::arg("err"));

@@ -29,22 +29,6 @@ class _Refuse(torch.autograd.Function):
         raise RuntimeError(f"{ctx.name} has no second derivative: its gradients are differentiable no further")
 
 
-class _Edge(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, t):
-        ctx.set_materialize_grads(False)
-        return t.new_empty(0)
-
-    @staticmethod
-    def backward(ctx, g):
-        return None
-
-
-def edge_of(t: torch.Tensor) -> torch.Tensor | None:
-    """An empty tensor with ``t``'s place in the graph, for a backward that needs ``t`` itself no more."""
-    return _Edge.apply(t) if torch.is_grad_enabled() and t.requires_grad else None
-
-
 def refuse_second(name: str, grads: tuple, *depends: torch.Tensor | None) -> tuple:
     """``grads`` (some may be None) as a backward returns them; differentiating them raises."""
     if not torch.is_grad_enabled():

@@ -30,7 +30,7 @@ from __future__ import annotations
 import torch
 
 from graspo_b200.ops._ext import err_word, ext, launches
-from graspo_b200.ops._second import edge_of, refuse_second
+from graspo_b200.ops._second import refuse_second
 
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
@@ -66,28 +66,27 @@ def _torch_loss(h, weight, targets, ignore_index, reduction):
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h, weight, targets, ignore_index, reduction, piece, h_edge=None):
+    def forward(ctx, h, weight, targets, ignore_index, reduction, piece):
         (loss, *state), count = ext().ce_forward(h, weight, targets, ignore_index, REDUCTIONS[reduction],
                                                  err_word(h.device))
         launches.add(count - 1)
-        ctx.save_for_backward(weight, h_edge, *state)
+        ctx.save_for_backward(weight, *state)
         ctx.shape, ctx.tokens, ctx.reduction, ctx.piece = h.shape, targets.numel(), reduction, piece
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        weight, h_edge, hc, state = ctx.saved_tensors
+        weight, hc, state, h_edge = ctx.saved_tensors
         (dh, dw), count = ext().ce_backward(hc, state, weight, ctx.tokens, g.float().contiguous().view(-1),
                                             REDUCTIONS[ctx.reduction], ctx.needs_input_grad[0],
                                             ctx.needs_input_grad[1], ctx.piece, err_word(hc.device))
         launches.add(count - 1)
         dh, dw = refuse_second("linear_cross_entropy", (None if dh is None else dh.view(ctx.shape), dw),
                                g, weight, h_edge)
-        return dh, dw, None, None, None, None, None
+        return dh, dw, None, None, None, None
 
 
-def _kernel_loss(h, weight, targets, ignore_index, reduction, piece):
-    return _LinearCrossEntropy.apply(h, weight, targets, ignore_index, reduction, piece, edge_of(h))
+_kernel_loss = _LinearCrossEntropy.apply
 
 
 def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,

@@ -405,8 +405,23 @@ def _ce_live(targets, V, ignore_index):
     return (targets != ignore_index) & (targets >= 0) & (targets < V)
 
 
+class _Edge(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, t):
+        ctx.set_materialize_grads(False)
+        return t.new_empty(0)
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
 def ce_forward(h, W, targets, ignore_index, reduction, err):
     """The state's tensors here are the trained rows and (position, target, lse, p - 1) of each."""
+    edge = None
+    if h.requires_grad:
+        with torch.enable_grad():
+            edge = _Edge.apply(h)
     t = targets.reshape(-1).long()
     live = _ce_live(t, W.shape[0], ignore_index)
     bad = ~live & (t != ignore_index)
@@ -423,8 +438,8 @@ def ce_forward(h, W, targets, ignore_index, reduction, err):
     loss[rows] = torch.logaddexp(torch.zeros(()), torch.logsumexp(lead, -1))
     state = torch.stack([rows.double(), t[rows].double(), lse.double(), torch.expm1(-loss[rows]).double()])
     if reduction == 0:
-        return (loss.view(targets.shape), hc, state), 1
-    return (loss.sum() / (max(1, rows.numel()) if reduction == 2 else 1), hc, state), 1
+        return (loss.view(targets.shape), hc, state, edge), 1
+    return (loss.sum() / (max(1, rows.numel()) if reduction == 2 else 1), hc, state, edge), 1
 
 
 def ce_backward(hc, state, W, tokens, grad, reduction, want_h, want_w, piece, err):
