@@ -11,7 +11,8 @@
 //             forward's loss in the target's column.
 //   kCeDh     rows tokens, columns hidden, K a vocabulary piece: fp32 sums of
 //             dh, K split into slices where there are few tiles.
-//   kCeDw     rows vocabulary, columns hidden, K the tokens: dW in bf16.
+//   kCeDw     rows vocabulary, columns hidden, K the tokens: dW in bf16, with what
+//             the rounding of d took from the targets' entries.
 //
 // One CTA per SM, 10 warps: TMA producer, MMA issuer, eight epilogue warps (two
 // per 32-lane quarter of the accumulator, 128 columns each).  Four epilogue warps
@@ -62,8 +63,24 @@ struct Args {
   int kb_first;           // kDh: K-blocks of the first piece, which fix the slices
   bool add;               // kDh: a later piece
   const float* unit;      // kDw: what the ratios are multiples of
+  const unsigned* sorted; // kDw: the tokens' targets in order,
+  const int* start;       //   where each 32 vocabulary rows start among them,
+  int row_blocks;         //   for so many of 32,
+  const float* rest;      //   and what a row lacks, at its first token and, not `joined`,
+  long ldr;               //   at every kGroup-th place of the order that is its too
+  bool joined;
   bool early;             // host: how the kernel is launched
 };
+
+constexpr int kGroup = 32;   // tokens, in the order of their targets, whose rests are added at once
+
+__host__ __device__ __forceinline__ long row_blocks(long V) { return (V + 31) / 32; }
+
+// What rounding the target's entry of d to bf16 leaves out.
+__device__ __forceinline__ float rounded_off(float d) {
+  const float rest = d - __bfloat162float(__float2bfloat16(d));
+  return fabsf(rest) < INFINITY ? rest : 0.f;   // an entry that is not finite stays what it is
+}
 
 // Slices that the reduction of dh is split into, none of them empty: as many as
 // fill the SMs, with at least four K-blocks each; with more tiles than SMs two
@@ -319,6 +336,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr float kLog2e = 1.4426950408889634f;
     const float unit = MODE == kDw ? __ldcg(args.unit) : 1.f;
     int acc_iter = 0;
+    // kDw: the first token of this lane's row in the order of the targets, -1 without one;
+    // found, and its rests fetched, during the unit before
+    int next_at = -1;
+    const auto look_up = [&](int u) {
+      const Unit w = decode_unit(u, num_m, num_n, 1, kb_total);
+      const unsigned row = static_cast<unsigned>(args.n_first + w.m_block * BM + quarter * 32 + lane);
+      const int block = min(static_cast<int>(row / 32), args.row_blocks);
+      int lo = args.start[block], hi = args.start[min(block + 1, args.row_blocks)];
+      const int past = hi;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (args.sorted[mid] < row) lo = mid + 1;
+        else hi = mid;
+      }
+      next_at = lo < past && args.sorted[lo] == row ? lo : -1;
+      if (next_at >= 0) {
+        const float* rest = args.rest + next_at * args.ldr + w.n_block * BN + half * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (w.n_block * BN + half * 128 + i * 32 < args.ldr)
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(rest + i * 32));
+      }
+    };
+    if constexpr (MODE == kDw)
+      if (static_cast<int>(blockIdx.x) < units) look_up(blockIdx.x);
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const Unit w = decode_unit(u, num_m, num_n, splits, kb_total);
       const int m = w.m_block * BM + quarter * 32 + lane;
@@ -387,6 +429,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
       } else {
         const int acc = acc_iter & 1;
+        const int token_at = next_at;
+        if constexpr (MODE == kDw)
+          if (u + static_cast<int>(gridDim.x) < units) look_up(u + gridDim.x);
         const bool have = mbar_wait(&tfull[acc], (acc_iter >> 1) & 1, args.err, kErrTmemFullTimeout);
         tc_fence_after();
 #pragma unroll 1
@@ -430,6 +475,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           } else if constexpr (MODE == kDw) {
+            if (token_at >= 0 && count > 0) {   // `rest` has whole lines
+              const unsigned row = static_cast<unsigned>(args.n_first + m);
+              int at = token_at;
+              do {
+                const float4* src = reinterpret_cast<const float4*>(args.rest + at * args.ldr + nc);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                  const float4 x = src[q];
+                  v[4 * q] += x.x, v[4 * q + 1] += x.y, v[4 * q + 2] += x.z, v[4 * q + 3] += x.w;
+                }
+                at = (at / kGroup + 1) * kGroup;
+              } while (!args.joined && at < live && args.sorted[at] == row);
+            }
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= unit;
             __nv_bfloat16* C = static_cast<__nv_bfloat16*>(args.C) + nc;

@@ -21,10 +21,12 @@
 // holds only without a factor that is common to all tokens: 1 / n times (p - 1)
 // would round the same way in every row that matters.  So s_t = unit * r_t, with
 // the largest |s_t| as the unit; d carries r_t (1 for a mean or a sum), and the
-// unit multiplies the fp32 sums.  What does not average out is r_t (p - 1) in a row
-// of dW that is the target of one or two tokens: with a weight per token the
-// gradients are 2.4e-3 of their norm off at 466 x 1000 x 50001, where rounding the
-// exact ones is 1.7e-3 (and a mean's are).
+// unit multiplies the fp32 sums.  Nor does r_t (p - 1) average out, in dh_t and in a
+// row of dW that is the target of a token or a few: what its rounding leaves out is
+// added to the fp32 sums: to dh_t where its row is put together (ce_scatter), to the
+// rows of dW in the product's epilogue, from sums by target (ce_rest).  Without it the gradients were 2.4e-3 of
+// their norm off with a weight per token at 466 x 1000 x 50001, where rounding the
+// exact ones is 1.7e-3.
 //
 // Bound by the tensor cores where there are many tokens.  Measured on a B200, loss
 // and both gradients: 6144 trained tokens x 4096 x 151936 25.9 ms (four products at
@@ -42,17 +44,30 @@
 
 namespace gb {
 
+// embedding_grad.cu: ids [0, vocab) sorted, ties by position, the others last; ints:
+// the ids, the positions, and as many of scratch.  Two launches (over 1024 tokens).
+void sort_tokens(const int64_t* ids, int64_t tokens, int64_t vocab, int64_t skip, int64_t ignore, int* ints, int* err,
+                 cudaStream_t stream);
+
 namespace {
 
 constexpr int kRowPad = BM;     // rows of the compacted buffers come in whole GEMM tiles,
 constexpr int kColumnPad = 64;  // and start on 128-byte lines
 constexpr int kBlock = 256;
 constexpr int kTokens = 32;     // tokens per block of ce_compact
+// Tokens up to which ce_finish ranks the targets by counting, the square of the tokens;
+// beyond, they are sorted, in three more launches.
+constexpr int64_t kRankTokens = 2048;
+// Tokens from which a row's rests are joined in a launch of their own; up to it dW's
+// epilogue adds at most kJoinTokens / kGroup + 1 of them.
+constexpr int64_t kJoinTokens = 256;
+constexpr int kRestThreads = 128, kRestColumns = kRestThreads * 8;
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 // What the forward leaves for the backward, in one int32 tensor.  `unit` and `ratio`
-// are those of an upstream gradient of 1; a backward of its own replaces them.
+// (and `rest`) are those of an upstream gradient of 1; a backward of its own replaces
+// them.
 struct State {
   int* count;           // number of trained tokens
   float* unit;          // what the tokens' weights are multiples of
@@ -63,7 +78,11 @@ struct State {
   float* ratio;         // its weight over the unit
   float* target_logit;
   float* hot;           // p - 1 of its target
-  static int64_t words(int64_t cap) { return 4 + 8 * cap; }
+  int* order;           // the trained tokens by target, equal ones in their order,
+  unsigned* sorted;     // and their targets,
+  float* rest;          // and what rounding their entry of d leaves out (over the unit)
+  int* start;           // [V / 32 + 1] where each 32 vocabulary rows' tokens start among them
+  static int64_t words(int64_t cap, int64_t V) { return 4 + 11 * cap + ce::row_blocks(V) + 1; }
   State(const torch::Tensor& t, int64_t cap) {
     int* p = t.data_ptr<int>();
     count = p;
@@ -75,6 +94,10 @@ struct State {
     ratio = lse + cap;
     target_logit = ratio + cap;
     hot = target_logit + cap;
+    order = reinterpret_cast<int*>(hot + cap);
+    sorted = reinterpret_cast<unsigned*>(order + cap);
+    rest = reinterpret_cast<float*>(sorted + cap);
+    start = reinterpret_cast<int*>(rest + cap);
   }
 };
 
@@ -197,40 +220,179 @@ __device__ __forceinline__ float common_weight(const float* g, bool mean, int n)
 // of the largest logit's last place, 2e-6 at 20 and 3e-5 at 300, where a confident
 // token's loss is 1e-6.)  p - 1 = expm1(-loss) likewise: exp(l - lse) - 1 from the
 // remade logit was off by 2.5e-5, a quarter of it at a loss of 1e-4.
+// Also the tokens by target (`rank`; else ce_list_kernel makes the list): a token's
+// place is the number of smaller targets, and of equal ones before it, which its warp
+// counts; a further warp counts for each start of 32 vocabulary rows.
 __global__ void __launch_bounds__(kBlock) ce_finish_kernel(const float2* part, int parts, State st,
-                                                             const float* __restrict__ g, bool mean,
-                                                             float* __restrict__ loss) {
+                                                             const float* __restrict__ g, bool mean, bool rank,
+                                                             int row_blocks, float* __restrict__ loss) {
   pdl_trigger();
   pdl_wait();
   const int n = *st.count;
   const int lane = threadIdx.x & 31;
   if (blockIdx.x == 0 && threadIdx.x == 0) *st.unit = common_weight(g, mean, n);
-  for (long m = blockIdx.x * (kBlock / 32L) + (threadIdx.x >> 5); m < n; m += gridDim.x * (kBlock / 32L)) {
-    const float2* row = part + m * parts;
-    float mx = -INFINITY, sum = 0.f;
+  const long items = n + (rank ? row_blocks + 1 : 0);
+  for (long m = blockIdx.x * (kBlock / 32L) + (threadIdx.x >> 5); m < items; m += gridDim.x * (kBlock / 32L)) {
+    float hot = 0.f;
+    if (m < n) {
+      const float2* row = part + m * parts;
+      float mx = -INFINITY, sum = 0.f;
 #pragma unroll 4
-    for (int b = lane; b < parts; b += 32) {
-      const float2 p = row[b];
-      const float top = fmaxf(mx, p.x);
-      if (top > -INFINITY) sum = sum * __expf(mx - top) + p.y * __expf(p.x - top);
-      else sum += p.y;  // a half tile of NaN only has a NaN sum and no maximum
-      mx = top;
-    }
-    const float top = warp_max(mx);
-    sum = warp_sum(top > -INFINITY ? sum * __expf(mx - top) : sum);
-    if (lane == 0) {
-      const float t = st.target_logit[m], rest = logf(sum);
-      const float z = (top - t) + rest;
+      for (int b = lane; b < parts; b += 32) {
+        const float2 p = row[b];
+        const float top = fmaxf(mx, p.x);
+        if (top > -INFINITY) sum = sum * __expf(mx - top) + p.y * __expf(p.x - top);
+        else sum += p.y;  // a half tile of NaN only has a NaN sum and no maximum
+        mx = top;
+      }
+      const float top = warp_max(mx);
+      sum = warp_sum(top > -INFINITY ? sum * __expf(mx - top) : sum);
+      const float t = st.target_logit[m], others = logf(sum);
+      const float z = (top - t) + others;
       const float q = log1pf(expf(-fabsf(z)));
       // an infinite logit of the target leaves no loss, as inf - inf; -inf gives inf, NaN stays NaN
       const bool lost = t == INFINITY;
-      st.lse[m] = lost ? __int_as_float(0x7fc00000) : z > 0.f ? (top + rest) + q : t + q;
-      st.ratio[m] = 1.f;
       const float l = lost ? __int_as_float(0x7fc00000) : fmaxf(z, 0.f) + q;
-      st.hot[m] = expm1f(-l);
-      loss[st.token[m]] = l;
+      hot = expm1f(-l);
+      if (lane == 0) {
+        st.lse[m] = lost ? l : z > 0.f ? (top + others) + q : t + q;
+        st.ratio[m] = 1.f;
+        st.hot[m] = hot;
+        loss[st.token[m]] = l;
+      }
+    }
+    if (!rank) continue;
+    const int64_t y = m < n ? st.target[m] : (m - n) * 32;
+    int place = 0;
+#pragma unroll 8
+    for (int k = lane; k < n; k += 32) {
+      const int64_t z = st.target[k];
+      place += z < y || (z == y && k < m && m < n);
+    }
+    place = __reduce_add_sync(0xffffffffu, place);
+    if (lane == 0) {
+      if (m < n) {
+        st.order[place] = static_cast<int>(m);
+        st.sorted[place] = static_cast<unsigned>(y);
+        st.rest[place] = ce::rounded_off(hot);
+      } else {
+        st.start[m - n] = place;
+      }
     }
   }
+}
+
+// The tokens by target from the sorted targets and their positions, whose first n are
+// the trained ones.
+__global__ void __launch_bounds__(kBlock) ce_list_kernel(const unsigned* __restrict__ by_id,
+                                                           const int* __restrict__ token_by_id, State st,
+                                                           int row_blocks) {
+  pdl_trigger();
+  const int n = *st.count;
+  const int first = blockIdx.x * kBlock + threadIdx.x, step = gridDim.x * kBlock;
+  for (int k = first; k < n; k += step) {
+    const int m = st.place[token_by_id[k]];
+    st.order[k] = m;
+    st.sorted[k] = by_id[k];
+    st.rest[k] = ce::rounded_off(st.hot[m]);
+  }
+  for (int b = first; b <= row_blocks; b += step) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (by_id[mid] < 32u * static_cast<unsigned>(b)) lo = mid + 1;
+      else hi = mid;
+    }
+    st.start[b] = lo;
+  }
+}
+
+// What rows of dW lack: sums of rest_t h_t over the tokens of a target, at its first
+// place in the order of the targets.  A block takes kGroup places and kRestColumns
+// columns, and leaves a sum at the first place of every target among them: a target
+// of many tokens has one per group (joined below), and no chain is longer than that.
+__global__ void __launch_bounds__(kRestThreads) ce_rest_kernel(const __nv_bfloat16* hc, int Hp, int slabs, State st,
+                                                               float* out) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int G = ce::kGroup, U = 8;
+  __shared__ int token[G];
+  __shared__ unsigned target[G];
+  __shared__ float rest[G];
+  const int n = *st.count;
+  const long first = static_cast<long>(blockIdx.x / slabs) * G;
+  if (first >= n) return;
+  const int count = static_cast<int>(min(static_cast<long>(G), n - first));
+  const int t = threadIdx.x;
+  if (t < count) {
+    token[t] = st.order[first + t];
+    target[t] = st.sorted[first + t];
+    rest[t] = st.rest[first + t];
+  }
+  __syncthreads();
+  const int column = static_cast<int>(blockIdx.x % slabs) * kRestColumns + t * 8;
+  if (column >= Hp) return;
+  float sum[8] = {};
+  int head = 0;
+  const auto flush = [&] {
+    store_pack<float, 8>(out + (first + head) * Hp + column, sum);
+  };
+#pragma unroll 1
+  for (int j0 = 0; j0 < count; j0 += U) {
+    Pack<__nv_bfloat16, 8> p[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (j0 + j < count) p[j] = load_raw<__nv_bfloat16, 8>(hc + static_cast<long>(token[j0 + j]) * Hp + column);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (j0 + j >= count) break;
+      if (target[j0 + j] != target[head]) {
+        flush();
+        head = j0 + j;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+      }
+      const float e = rest[j0 + j];
+      if (e != 0.f)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = fmaf(e, value(p[j], i), sum[i]);
+    }
+  }
+  flush();
+}
+
+// Joins the sums of targets that go on past a group, onto the first of them; the block
+// of the first group that a target goes on into does it.
+__global__ void __launch_bounds__(kRestThreads) ce_join_kernel(int Hp, int slabs, State st, float* sums) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int G = ce::kGroup, U = 8;
+  const int n = *st.count;
+  const long first = static_cast<long>(blockIdx.x / slabs) * G;
+  if (first == 0 || first >= n) return;
+  const unsigned target = st.sorted[first];
+  if (st.sorted[first - 1] != target || (first > G && st.sorted[first - G - 1] == target)) return;
+  const int column = static_cast<int>(blockIdx.x % slabs) * kRestColumns + static_cast<int>(threadIdx.x) * 8;
+  if (column >= Hp) return;
+  long head = first - 1;   // the target's first place
+  while (head > first - G && st.sorted[head - 1] == target) --head;
+  float sum[8];
+  load_pack<float, 8>(sums + head * Hp + column, sum);
+  for (long k0 = first; k0 < n && st.sorted[k0] == target; k0 += U * G) {
+    Pack<float, 8> p[U];
+    bool some[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      some[j] = k0 + j * G < n && st.sorted[k0 + j * G] == target;
+      if (some[j]) p[j] = load_raw<float, 8>(sums + (k0 + j * G) * Hp + column);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (some[j])
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += value(p[j], i);
+  }
+  store_pack<float, 8>(sums + head * Hp + column, sum);
 }
 
 // Unit and ratios from an upstream gradient per token (the unit is the largest
@@ -256,6 +418,10 @@ __global__ void __launch_bounds__(1024) ce_weight_kernel(const float* __restrict
   const float unit = top > 0.f ? top : 1.f;
   if (threadIdx.x == 0) *st.unit = unit;
   for (int m = threadIdx.x; m < n; m += 1024) st.ratio[m] = g[st.token[m]] / unit;
+  for (int k = threadIdx.x; k < n; k += 1024) {
+    const int m = st.order[k];
+    st.rest[k] = ce::rounded_off(g[st.token[m]] / unit * st.hot[m]);
+  }
 }
 
 // Sum of the tokens' losses in a fixed order, over the trained tokens for the
@@ -283,11 +449,12 @@ __global__ void __launch_bounds__(kBlock) ce_total_kernel(const float* loss, lon
   total_loss(loss, T, *st.count, mean, out);
 }
 
-// dh[t] = unit * sum of the slices' row place[t], rounded once; zero for an
-// ignored token.  A last block adds the losses up where `total` wants them.
+// dh[t] = unit * (sum of the slices' row place[t], and what the rounding of d left out
+// of the target's entry times its row of W), rounded once; zero for an ignored token.  A last block adds the losses up where `total` wants them.
 template <bool WIDE>
 __global__ void __launch_bounds__(kBlock) ce_scatter_kernel(const float* acc, int lda, State st, long T,
                                                               int H, int kb_first, int sms,
+                                                              const __nv_bfloat16* W, long ldw,
                                                               __nv_bfloat16* __restrict__ dh,
                                                               const float* loss, bool mean,
                                                               float* __restrict__ total) {
@@ -319,8 +486,11 @@ __global__ void __launch_bounds__(kBlock) ce_scatter_kernel(const float* acc, in
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] += f[j];
       }
+      const float rest = ce::rounded_off(st.ratio[m] * st.hot[m]);
+      float row[V];
+      load_pack<__nv_bfloat16, V>(W + st.target[m] * ldw + c, row);
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[j] *= unit;
+      for (int j = 0; j < V; ++j) s[j] = (rest != 0.f ? fmaf(rest, row[j], s[j]) : s[j]) * unit;
     }
     store_pack<__nv_bfloat16, V>(dh + t * H + c, s);
   }
@@ -382,7 +552,7 @@ Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Ten
   const int num_n = static_cast<int>((f.V + ce::BN - 1) / ce::BN);
   const auto f32 = h.options().dtype(torch::kFloat32);
   f.loss = torch::empty({f.T}, f32);
-  f.state = torch::empty({State::words(f.cap)}, h.options().dtype(torch::kInt32));
+  f.state = torch::empty({State::words(f.cap, f.V)}, h.options().dtype(torch::kInt32));
   f.hc = torch::empty({f.cap, f.Hp}, h.options());
   torch::Tensor part = torch::empty({f.cap, 2 * num_n, 2}, f32);
   const State st(f.state, f.cap);
@@ -407,10 +577,20 @@ Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Ten
   args.target_logit = st.target_logit;
   ce::launch<ce::kLse, 0>(make_tmap_bf16(f.hc.data_ptr(), f.cap, f.Hp, f.Hp, BM),
                           make_tmap_bf16(f.W.data_ptr(), f.V, f.H, f.W.stride(0), ce::BN), args, stream, device);
-  ce::launch_chained(args.early, ce_finish_kernel, static_cast<unsigned>(std::min<int64_t>((f.cap + 7) / 8, 148 * 8)), kBlock, 0,
-                     stream, static_cast<const float2*>(args.part), 2 * num_n, st, grad, reduction == kMean,
+  const bool rank = f.T <= kRankTokens;
+  const int row_blocks = static_cast<int>(ce::row_blocks(f.V));
+  ce::launch_chained(args.early, ce_finish_kernel,
+                     static_cast<unsigned>(std::min<int64_t>((f.cap + row_blocks + 8) / 8, 148 * 8)), kBlock, 0, stream,
+                     static_cast<const float2*>(args.part), 2 * num_n, st, grad, reduction == kMean, rank, row_blocks,
                      f.loss.data_ptr<float>());
-  f.launches = 3 + !f.W.is_same(W);
+  if (!rank) {
+    torch::Tensor sorted = torch::empty({4 * f.T}, f.state.options());
+    int* ints = sorted.data_ptr<int>();
+    sort_tokens(targets.data_ptr<int64_t>(), f.T, f.V, ignore_index, ignore_index, ints, err, stream);
+    ce_list_kernel<<<148 * 4, kBlock, 0, stream>>>(reinterpret_cast<const unsigned*>(ints), ints + f.T, st, row_blocks);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  f.launches = 3 + !f.W.is_same(W) + (rank ? 0 : 3);
   return f;
 }
 
@@ -432,9 +612,22 @@ int64_t backward(const torch::Tensor& hc, const State& st, const torch::Tensor& 
   const int64_t num_n = (H + ce::BN - 1) / ce::BN;
   const int sms = num_sms(device);
   const int kb_first = static_cast<int>((std::min(piece, V) + BK - 1) / BK);
-  torch::Tensor acc;  // room for the slices of any number of trained tokens (dh_slices)
-  if (dh != nullptr)
-    acc = torch::empty({std::max<int64_t>(sms / num_n, 2 * cap / BM) * BM * Hp}, hc.options().dtype(torch::kFloat32));
+  // room for dh's slices of any number of trained tokens (dh_slices), then what rows of dW lack
+  const int64_t acc_rows = dh != nullptr ? std::max<int64_t>(sms / num_n, 2 * cap / BM) * BM : 0;
+  const torch::Tensor sums =
+      torch::empty({acc_rows + (dW != nullptr ? cap : 0), Hp}, hc.options().dtype(torch::kFloat32));
+  float* acc = sums.data_ptr<float>();
+  float* rests = acc + acc_rows * Hp;
+  const bool join = T > kJoinTokens;
+  if (dW != nullptr) {
+    const unsigned slabs = static_cast<unsigned>((Hp + kRestColumns - 1) / kRestColumns);
+    ce::launch_chained(early, ce_rest_kernel, static_cast<unsigned>(cap / ce::kGroup) * slabs, kRestThreads, 0, stream,
+                       static_cast<const __nv_bfloat16*>(ptr<__nv_bfloat16>(hc)), static_cast<int>(Hp),
+                       static_cast<int>(slabs), st, rests);
+    if (join)
+      ce::launch_chained(early, ce_join_kernel, static_cast<unsigned>(cap / ce::kGroup) * slabs, kRestThreads, 0, stream,
+                         static_cast<int>(Hp), static_cast<int>(slabs), st, rests);
+  }
   const CUtensorMap map_h = make_tmap_bf16(hc.data_ptr(), cap, Hp, Hp, BM);
   const CUtensorMap map_h_mn = make_tmap_bf16(hc.data_ptr(), cap, Hp, Hp, 64);
   for (int64_t v0 = 0; v0 < V; v0 += piece) {
@@ -460,7 +653,7 @@ int64_t backward(const torch::Tensor& hc, const State& st, const torch::Tensor& 
       a.N = static_cast<int>(H);
       a.kb = static_cast<int>((nv + BK - 1) / BK);
       a.kb_first = kb_first;
-      a.C = acc.data_ptr();
+      a.C = acc;
       a.ldc = Hp;
       a.add = v0 > 0;
       ce::launch<ce::kDh, 1>(make_tmap_bf16(d.data_ptr(), cap, nv, piece, BM),
@@ -474,6 +667,12 @@ int64_t backward(const torch::Tensor& hc, const State& st, const torch::Tensor& 
       a.C = ptr<__nv_bfloat16>(*dW) + v0 * H;
       a.ldc = H;
       a.unit = st.unit;
+      a.sorted = st.sorted;
+      a.start = st.start;
+      a.rest = rests;
+      a.ldr = Hp;
+      a.joined = join;
+      a.row_blocks = static_cast<int>(ce::row_blocks(V));
       ce::launch<ce::kDw, 3>(make_tmap_bf16(d.data_ptr(), cap, nv, piece, 64), map_h_mn, a, stream, device);
     }
   }
@@ -482,13 +681,14 @@ int64_t backward(const torch::Tensor& hc, const State& st, const torch::Tensor& 
     const int rows = static_cast<int>(std::max<int64_t>(std::min<int64_t>(T * per_row, 148 * 16), 1));
     ce::launch_chained(early, H % 8 == 0 ? ce_scatter_kernel<true> : ce_scatter_kernel<false>,
                        rows + (total != nullptr ? 1 : 0), kBlock, 0, stream,
-                       static_cast<const float*>(acc.data_ptr<float>()), static_cast<int>(Hp), st, static_cast<long>(T),
-                       static_cast<int>(H), kb_first, sms, ptr<__nv_bfloat16>(*dh),
+                       static_cast<const float*>(acc), static_cast<int>(Hp), st, static_cast<long>(T),
+                       static_cast<int>(H), kb_first, sms, static_cast<const __nv_bfloat16*>(ptr<__nv_bfloat16>(W)),
+                       static_cast<long>(W.stride(0)), ptr<__nv_bfloat16>(*dh),
                        static_cast<const float*>(loss.defined() ? loss.data_ptr<float>() : nullptr), mean,
                        total != nullptr ? total->data_ptr<float>() : nullptr);
   }
   const int64_t pieces = (V + piece - 1) / piece, each = 1 + (dh != nullptr) + (dW != nullptr);
-  return pieces * each + (dh != nullptr);
+  return pieces * each + (dh != nullptr) + (dW != nullptr ? 1 + join : 0);
 }
 
 void check_inputs(const torch::Tensor& h, const torch::Tensor& W, const torch::Tensor& targets, int64_t reduction) {
@@ -544,7 +744,7 @@ Launched ce_forward(torch::Tensor h, torch::Tensor W, torch::Tensor targets, int
 Launched ce_backward(torch::Tensor hc, torch::Tensor state, torch::Tensor W, int64_t tokens, torch::Tensor grad,
                      int64_t reduction, bool want_h, bool want_w, int64_t piece, torch::Tensor err) {
   const int64_t H = W.size(1), V = W.size(0), cap = capacity(tokens);
-  require(hc.is_cuda() && hc.size(0) == cap && hc.size(1) == round_up(H, kColumnPad) && state.numel() == State::words(cap),
+  require(hc.is_cuda() && hc.size(0) == cap && hc.size(1) == round_up(H, kColumnPad) && state.numel() == State::words(cap, V),
           "state of another call");
   check_piece(piece);
   const float* g = check_grad(grad, hc, reduction, tokens);
@@ -554,9 +754,12 @@ Launched ce_backward(torch::Tensor hc, torch::Tensor state, torch::Tensor W, int
   if (!want_h && !want_w) return {{dh, dW}, 0};
   // two backward passes of one graph may run at once: the weights are this call's own
   State st(state, cap);
-  torch::Tensor weights = torch::empty({4 + (reduction == kNone ? cap : 0)}, hc.options().dtype(torch::kFloat32));
+  torch::Tensor weights = torch::empty({4 + (reduction == kNone ? 2 * cap : 0)}, hc.options().dtype(torch::kFloat32));
   st.unit = weights.data_ptr<float>();
-  if (reduction == kNone) st.ratio = st.unit + 4;
+  if (reduction == kNone) {
+    st.ratio = st.unit + 4;
+    st.rest = st.ratio + cap;
+  }
   ce_weight_kernel<<<1, 1024, 0, stream>>>(g, reduction == kNone, reduction == kMean, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (want_h) dh = torch::empty({tokens, H}, hc.options());

@@ -130,10 +130,12 @@ __device__ __forceinline__ Key sort_keys(Key k, Key (&s)[2][kSortKeys], int& fli
 }
 
 // Sorted chunks of (id, place in the chunk).  Padding ids, and ids outside the
-// table (reported), become the largest id, kNoId in the output.
+// table (reported unless they are `ignore`), become the largest id, kNoId in the
+// output.
 template <typename Key>
 __global__ void __launch_bounds__(kSortKeys) embed_sort_kernel(const int64_t* __restrict__ ids, long tokens, long V,
-                                                               long padding, unsigned* __restrict__ id_out,
+                                                               long padding, long ignore,
+                                                               unsigned* __restrict__ id_out,
                                                                int* __restrict__ token_out, int* __restrict__ err) {
   constexpr int kPlaceBits = 10;
   constexpr Key kNone = ~Key(0) >> kPlaceBits;
@@ -146,8 +148,11 @@ __global__ void __launch_bounds__(kSortKeys) embed_sort_kernel(const int64_t* __
   if (t < n) {
     const long id = ids[base + t];
     Key u = kNone;
-    if (id < 0 || id >= V) atomicExch(err + 1, kErrBadToken);
-    else if (id != padding) u = static_cast<Key>(id);
+    if (id >= 0 && id < V) {
+      if (id != padding) u = static_cast<Key>(id);
+    } else if (id != ignore) {
+      atomicExch(err + 1, kErrBadToken);
+    }
     k = u << kPlaceBits | static_cast<Key>(t);
   }
   int flip = 0;
@@ -489,6 +494,29 @@ unsigned blocks_for(long a, long b) {
 
 }  // namespace
 
+// ids [0, vocab) sorted, ties by position, `skip` and ids outside (reported unless
+// they are `ignore`) last as kNoId.  ints: the ids, the positions, and for more than
+// kSortKeys tokens as many of scratch (the sorted chunks before their merge).  One
+// launch, or two.
+void sort_tokens(const int64_t* ids, int64_t tokens, int64_t vocab, int64_t skip, int64_t ignore, int* ints, int* err,
+                 cudaStream_t stream) {
+  const bool one = tokens <= kSortKeys;
+  unsigned* id = reinterpret_cast<unsigned*>(ints);
+  int* token = ints + tokens;
+  unsigned* id_chunks = one ? id : reinterpret_cast<unsigned*>(ints + 2 * tokens);
+  int* token_chunks = one ? token : ints + 3 * tokens;
+  // 32-bit keys hold 10 bits of place and 22 of the id, whose last value is kept
+  (vocab < (1L << 22) ? embed_sort_kernel<unsigned> : embed_sort_kernel<unsigned long long>)<<<
+      blocks_for(tokens, kSortKeys), kSortKeys, 0, stream>>>(ids, tokens, vocab, skip, ignore, id_chunks,
+                                                             token_chunks, err);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (!one) {
+    embed_merge_kernel<<<blocks_for(tokens, 32), kThreads, 0, stream>>>(id_chunks, token_chunks,
+                                                                        static_cast<int>(tokens), id, token);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+}
+
 torch::Tensor embed_fwd(torch::Tensor ids, torch::Tensor table, double scale, torch::Tensor err) {
   require(table.is_cuda() && is_storage_type(table) && table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1 &&
               table.size(1) < (1L << 30),
@@ -548,19 +576,8 @@ torch::Tensor embed_bwd(torch::Tensor dy, torch::Tensor ids, int64_t vocab, c10:
   int* at = ints.data_ptr<int>();
   unsigned* id = reinterpret_cast<unsigned*>(at);
   int* token = at + tokens;
-  unsigned* id_chunks = one ? id : reinterpret_cast<unsigned*>(at + 2 * tokens);
-  int* token_chunks = one ? token : at + 3 * tokens;
   int* start = at + (one ? 2 : 4) * tokens;
-  // 32-bit keys hold 10 bits of place and 22 of the id, whose last value is kept
-  (vocab < (1L << 22) ? embed_sort_kernel<unsigned> : embed_sort_kernel<unsigned long long>)<<<
-      blocks_for(tokens, kSortKeys), kSortKeys, 0, stream>>>(flat.data_ptr<int64_t>(), tokens, vocab, padding,
-                                                             id_chunks, token_chunks, err.data_ptr<int>());
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  if (!one) {
-    embed_merge_kernel<<<blocks_for(tokens, 32), kThreads, 0, stream>>>(id_chunks, token_chunks,
-                                                                        static_cast<int>(tokens), id, token);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-  }
+  sort_tokens(flat.data_ptr<int64_t>(), tokens, vocab, padding, /*ignore (none)=*/0, at, err.data_ptr<int>(), stream);
   if (whole) {
     embed_start_kernel<<<blocks_for(vocab + 1, kThreads), kThreads, 0, stream>>>(id, static_cast<int>(tokens),
                                                                                  static_cast<int>(vocab), start);

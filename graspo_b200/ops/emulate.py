@@ -454,7 +454,8 @@ def ce_backward(hc, state, W, tokens, grad, reduction, want_h, want_w, piece, er
         Wv = _f(W[v0 : v0 + (piece or V)])
         hot = target[:, None] == torch.arange(v0, v0 + Wv.shape[0])
         p = torch.where(hot, state[3].float()[:, None], torch.exp(h @ Wv.T - lse[:, None]))
-        d = (ratio[:, None] * p).to(hc.dtype).float()
+        exact = ratio[:, None] * p
+        d = torch.where(hot, exact, exact.to(hc.dtype).float())  # the kernels add what the rounding leaves out
         acc += d @ Wv
         dw[v0 : v0 + Wv.shape[0]] = (d.T @ h * unit).to(dw.dtype)
     dh = torch.zeros(tokens, H, dtype=hc.dtype)

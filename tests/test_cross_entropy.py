@@ -569,13 +569,43 @@ def test_every_launch_is_counted(H, piece, copies, pieces):
         out = call()
         return launches.count - before, out
 
-    # compaction, (a copy of W's odd rows), product, row sums; per piece of the vocabulary the products; the rows of dh
+    # compaction, (a copy of W's odd rows), product, row sums; per piece of the vocabulary the products; the rows of
+    # dh; two for the sums that dW's rows lack
     forward = 3 + copies
-    assert counted(lambda: linear_cross_entropy_grads(h, w, t, piece=piece))[0] == forward + 3 * pieces + 1
+    assert counted(lambda: linear_cross_entropy_grads(h, w, t, piece=piece))[0] == forward + 3 * pieces + 3
     assert counted(lambda: linear_cross_entropy_grads(h, w, t, piece=piece, weight_grad=False))[0] == forward + 2 * pieces + 1
     assert counted(lambda: linear_cross_entropy_grads(h, w, t, grad=up, reduction="none", piece=piece))[0] == (
-        forward + 1 + 3 * pieces + 1)
+        forward + 1 + 3 * pieces + 3)
     hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
     n, loss = counted(lambda: linear_cross_entropy(hl, wl, t, piece=piece))
     assert n == forward + 1                                   # and the total
-    assert counted(loss.backward)[0] == 1 + copies + 3 * pieces + 1
+    assert counted(loss.backward)[0] == 1 + copies + 3 * pieces + 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,V,common", [(300, 264, 20011, 0.0), (61, 512, 4096, 0.0), (777, 1001, 5000, 0.4), (1, 72, 900, 0.0),
+                                          (2500, 136, 3000, 0.0), (700, 2056, 30000, 0.1)])
+def test_weights_per_token_are_not_rounded(T, H, V, common):
+    """The target's entry r (p - 1) carries no rounding to bf16: dh and dW are off by the rounding of the result (2^-8),
+    the errors of logits and exponentials, and the rounding of the other entries, which are sums over p.  In the norm
+    that is the error of rounding the exact result, where p is spread over the vocabulary (its square is below a tenth
+    of 1)."""
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy_grads
+
+    h, w, t, up = _case(T, H, V, 1.0, seed=T + V)
+    t[torch.rand(T, generator=torch.Generator().manual_seed(3)).cuda() < common] = 17       # one frequent target
+    _, dh, dw = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none")
+    _, wh, ww, _ = _oracle(h, w, t, up)
+    hd, wd, s = h.double(), w.double(), up.double().abs()[:, None]
+    p = torch.softmax(hd @ wd.T, -1)
+    delta = (H / 16 + 16) * 2.0 ** -22 * float((hd.abs() @ wd.abs().T).max())
+    hot = torch.zeros_like(p).scatter_(1, t[:, None], 1.0)
+    rel = (2.0 ** -8 + 3 * delta + 2.0 ** -17) * (1 + 2.0 ** -8)
+    exact = 4 * delta + 2.0 ** -15
+    err = (p * (1 - hot) * rel + hot * exact) * s
+    _within(dh, wh, err @ wd.abs() + 2.0 ** -8 * wh.abs() * (1 + 2.0 ** -8) + 1e-30, "dh")
+    _within(dw, ww, err.T @ hd.abs() + 2.0 ** -8 * ww.abs() * (1 + 2.0 ** -8) + 1e-30, "dw")
+    if T > 1:
+        for got, want in ((dh, wh), (dw, ww)):
+            best = (want.to(torch.bfloat16).double() - want).norm()
+            assert float((got.double() - want).norm()) <= 1.12 * float(best)
