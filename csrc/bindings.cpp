@@ -99,7 +99,7 @@ void adamw(torch::Tensor p, torch::Tensor g, torch::Tensor m, torch::Tensor v, d
 void transpose_bf16(torch::Tensor in, torch::Tensor out);
 using Launched = std::pair<std::vector<torch::Tensor>, int64_t>;
 Launched ce_forward(torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index, int64_t reduction,
-                    torch::Tensor err);
+                    bool want_w, torch::Tensor err);
 Launched ce_backward(torch::Tensor hc, torch::Tensor state, torch::Tensor W, int64_t tokens, torch::Tensor grad,
                      int64_t reduction, bool want_h, bool want_w, int64_t piece, torch::Tensor err);
 Launched ce_grads(torch::Tensor h, torch::Tensor W, torch::Tensor targets, c10::optional<torch::Tensor> grad,
@@ -225,13 +225,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("transpose_bf16", &gb::transpose_bf16);
   m.def("ce_forward",
         [](torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index, int64_t reduction,
-           torch::Tensor err) {
-          gb::Launched r = gb::ce_forward(h, W, targets, ignore_index, reduction, err);
+           bool want_w, torch::Tensor err) {
+          gb::Launched r = gb::ce_forward(h, W, targets, ignore_index, reduction, want_w, err);
           r.first.push_back(edge_of(h));
           return r;
         },
         "cross entropy over a vocabulary projection: (loss, state of its backward, the place of h in the graph), launches",
-        py::arg("h"), py::arg("W"), py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"), py::arg("err"));
+        py::arg("h"), py::arg("W"), py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"),
+        py::arg("want_w"), py::arg("err"));
   m.def("ce_backward", &gb::ce_backward, "(gradients of the cross entropy, in pieces of the vocabulary), launches", py::arg("hc"),
         py::arg("state"), py::arg("W"), py::arg("tokens"), py::arg("grad"), py::arg("reduction"), py::arg("want_h"),
         py::arg("want_w"), py::arg("piece"), py::arg("err"));

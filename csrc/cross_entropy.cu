@@ -397,7 +397,8 @@ __global__ void __launch_bounds__(kRestThreads) ce_join_kernel(int Hp, int slabs
 
 // Unit and ratios from an upstream gradient per token (the unit is the largest
 // finite size, 1 where there is none), or the unit of a reduced loss.
-__global__ void __launch_bounds__(1024) ce_weight_kernel(const float* __restrict__ g, bool per_token, bool mean, State st) {
+__global__ void __launch_bounds__(1024) ce_weight_kernel(const float* __restrict__ g, bool per_token, bool mean, bool ordered,
+                                                         State st) {
   pdl_trigger();
   pdl_wait();
   __shared__ float part[32];
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(1024) ce_weight_kernel(const float* __restrict
   const float unit = top > 0.f ? top : 1.f;
   if (threadIdx.x == 0) *st.unit = unit;
   for (int m = threadIdx.x; m < n; m += 1024) st.ratio[m] = g[st.token[m]] / unit;
-  for (int k = threadIdx.x; k < n; k += 1024) {
+  for (int k = threadIdx.x; ordered && k < n; k += 1024) {
     const int m = st.order[k];
     st.rest[k] = ce::rounded_off(g[st.token[m]] / unit * st.hot[m]);
   }
@@ -544,7 +545,7 @@ struct Forward {
 };
 
 Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Tensor& targets, int64_t ignore_index,
-                const float* grad, int64_t reduction, int* err, cudaStream_t stream) {
+                const float* grad, int64_t reduction, bool want_w, int* err, cudaStream_t stream) {
   Forward f;
   const int device = h.get_device();
   f.T = targets.numel(), f.H = W.size(1), f.V = W.size(0);
@@ -577,20 +578,21 @@ Forward forward(const torch::Tensor& h, const torch::Tensor& W, const torch::Ten
   args.target_logit = st.target_logit;
   ce::launch<ce::kLse, 0>(make_tmap_bf16(f.hc.data_ptr(), f.cap, f.Hp, f.Hp, BM),
                           make_tmap_bf16(f.W.data_ptr(), f.V, f.H, f.W.stride(0), ce::BN), args, stream, device);
-  const bool rank = f.T <= kRankTokens;
+  // the tokens by target, for dW
+  const bool rank = want_w && f.T <= kRankTokens, sort = want_w && !rank;
   const int row_blocks = static_cast<int>(ce::row_blocks(f.V));
   ce::launch_chained(args.early, ce_finish_kernel,
                      static_cast<unsigned>(std::min<int64_t>((f.cap + row_blocks + 8) / 8, 148 * 8)), kBlock, 0, stream,
                      static_cast<const float2*>(args.part), 2 * num_n, st, grad, reduction == kMean, rank, row_blocks,
                      f.loss.data_ptr<float>());
-  if (!rank) {
+  if (sort) {
     torch::Tensor sorted = torch::empty({4 * f.T}, f.state.options());
     int* ints = sorted.data_ptr<int>();
     sort_tokens(targets.data_ptr<int64_t>(), f.T, f.V, ignore_index, ignore_index, ints, err, stream);
     ce_list_kernel<<<148 * 4, kBlock, 0, stream>>>(reinterpret_cast<const unsigned*>(ints), ints + f.T, st, row_blocks);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
-  f.launches = 3 + !f.W.is_same(W) + (rank ? 0 : 3);
+  f.launches = 3 + !f.W.is_same(W) + (sort ? 3 : 0);
   return f;
 }
 
@@ -724,13 +726,14 @@ torch::Tensor flat_targets(const torch::Tensor& t) {
 // Each with the number of kernels launched.
 using Launched = std::pair<std::vector<torch::Tensor>, int64_t>;
 
-// (loss, compacted h, state): what ce_backward needs.
-Launched ce_forward(torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index,
-                                      int64_t reduction, torch::Tensor err) {
+// (loss, compacted h, state): what ce_backward needs; `want_w`: whether for dW too.
+Launched ce_forward(torch::Tensor h, torch::Tensor W, torch::Tensor targets, int64_t ignore_index, int64_t reduction,
+                    bool want_w, torch::Tensor err) {
   check_inputs(h, W, targets, reduction);
   const c10::cuda::CUDAGuard guard(h.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  const Forward f = forward(h, W, flat_targets(targets), ignore_index, nullptr, reduction, err.data_ptr<int>(), stream);
+  const Forward f = forward(h, W, flat_targets(targets), ignore_index, nullptr, reduction, want_w,
+                            err.data_ptr<int>(), stream);
   if (reduction == kNone) return {{f.loss.view(targets.sizes()), f.hc, f.state}, f.launches};
   torch::Tensor total = torch::empty({}, f.loss.options());
   ce_total_kernel<<<1, kBlock, 0, stream>>>(f.loss.data_ptr<float>(), f.T, State(f.state, f.cap), reduction == kMean,
@@ -760,7 +763,7 @@ Launched ce_backward(torch::Tensor hc, torch::Tensor state, torch::Tensor W, int
     st.ratio = st.unit + 4;
     st.rest = st.ratio + cap;
   }
-  ce_weight_kernel<<<1, 1024, 0, stream>>>(g, reduction == kNone, reduction == kMean, st);
+  ce_weight_kernel<<<1, 1024, 0, stream>>>(g, reduction == kNone, reduction == kMean, want_w, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (want_h) dh = torch::empty({tokens, H}, hc.options());
   if (want_w) dW = torch::empty({V, H}, hc.options());
@@ -779,12 +782,13 @@ Launched ce_grads(torch::Tensor h, torch::Tensor W, torch::Tensor targets, c10::
   const c10::cuda::CUDAGuard guard(h.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   int* e = err.data_ptr<int>();
-  const Forward f = forward(h, W, flat_targets(targets), ignore_index, reduction == kNone ? nullptr : g, reduction, e,
-                            stream);
+  const Forward f = forward(h, W, flat_targets(targets), ignore_index, reduction == kNone ? nullptr : g, reduction, want_w,
+                            e, stream);
   const State st(f.state, f.cap);
   const bool weighted = reduction == kNone && g != nullptr;
   if (weighted) {
-    ce::launch_chained(launches_early(f.cap, f.V, f.H), ce_weight_kernel, 1, 1024, 0, stream, g, true, false, st);
+    ce::launch_chained(launches_early(f.cap, f.V, f.H), ce_weight_kernel, 1, 1024, 0, stream, g, true, false, want_w,
+                       st);
   }
   torch::Tensor dh = torch::empty(h.sizes(), h.options()), dW, total;
   if (want_w) dW = torch::empty({f.V, f.H}, h.options());

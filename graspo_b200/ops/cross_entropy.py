@@ -68,7 +68,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, weight, targets, ignore_index, reduction, piece):
         (loss, *state), count = ext().ce_forward(h, weight, targets, ignore_index, REDUCTIONS[reduction],
-                                                 err_word(h.device))
+                                                 ctx.needs_input_grad[1], err_word(h.device))
         launches.add(count - 1)
         ctx.save_for_backward(weight, *state)
         ctx.shape, ctx.tokens, ctx.reduction, ctx.piece = h.shape, targets.numel(), reduction, piece

@@ -416,7 +416,7 @@ class _Edge(torch.autograd.Function):
         return None
 
 
-def ce_forward(h, W, targets, ignore_index, reduction, err):
+def ce_forward(h, W, targets, ignore_index, reduction, want_w, err):
     """The state's tensors here are the trained rows and (position, target, lse, p - 1) of each."""
     edge = None
     if h.requires_grad:

@@ -609,3 +609,22 @@ def test_weights_per_token_are_not_rounded(T, H, V, common):
         for got, want in ((dh, wh), (dw, ww)):
             best = (want.to(torch.bfloat16).double() - want).norm()
             assert float((got.double() - want).norm()) <= 1.12 * float(best)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [40, 300, 2300])
+@pytest.mark.parametrize("frozen", [None, "h", "w"])
+def test_autograd_gives_what_one_call_gives(T, frozen):
+    """The tokens by target are ranked, or sorted, for dW only; both forms have the same kernels."""
+    from graspo_b200.ops._ext import check_errors
+    from graspo_b200.ops.cross_entropy import linear_cross_entropy, linear_cross_entropy_grads
+
+    h, w, t, up = _case(T, 136, 900, 0.8, seed=T + 2)
+    want = linear_cross_entropy_grads(h, w, t, grad=up, reduction="none", weight_grad=frozen != "w")
+    hl, wl = h.clone().requires_grad_(frozen != "h"), w.clone().requires_grad_(frozen != "w")
+    loss = linear_cross_entropy(hl, wl, t, reduction="none")
+    loss.backward(up)
+    assert torch.equal(loss.detach(), want[0])
+    assert hl.grad is None if frozen == "h" else torch.equal(hl.grad, want[1])
+    assert wl.grad is None if frozen == "w" else torch.equal(wl.grad, want[2])
+    check_errors()
