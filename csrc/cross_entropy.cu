@@ -27,10 +27,14 @@
 // rows of dW in the product's epilogue, from sums by target (ce_rest).  Without it the gradients were 2.4e-3 of
 // their norm off with a weight per token at 466 x 1000 x 50001, where rounding the
 // exact ones is 1.7e-3.
+// The order of the targets, the sums and their addition cost 9 us at 61 x 512 x 4096,
+// 14 at 466 x 1000 x 50001 (whatever the targets: all in one row, or none twice) and
+// 0.1 ms at 6144 x 4096 x 151936.
 //
 // Bound by the tensor cores where there are many tokens.  Measured on a B200, loss
-// and both gradients: 6144 trained tokens x 4096 x 151936 25.9 ms (four products at
-// 1180 TFLOP/s under the power cap), 466 x 1000 x 50001 0.29 ms, 61 x 512 x 4096 40 us.
+// and both gradients: 6144 trained tokens x 4096 x 151936 25.6 to 26.5 ms (four
+// products at 1180 TFLOP/s under the power cap), 466 x 1000 x 50001 0.30 ms, 61 x 512 x
+// 4096 49 us.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -55,8 +59,9 @@ constexpr int kRowPad = BM;     // rows of the compacted buffers come in whole G
 constexpr int kColumnPad = 64;  // and start on 128-byte lines
 constexpr int kBlock = 256;
 constexpr int kTokens = 32;     // tokens per block of ce_compact
-// Tokens up to which ce_finish ranks the targets by counting, the square of the tokens;
-// beyond, they are sorted, in three more launches.
+// Tokens up to which ce_finish ranks the targets by counting, the square of the tokens
+// (3 us of 9 at 2048 tokens, 40 of 44 at 8192); beyond, they are sorted, in three more
+// launches (14 us at 2049, 17 at 8192).
 constexpr int64_t kRankTokens = 2048;
 // Tokens from which a row's rests are joined in a launch of their own; up to it dW's
 // epilogue adds at most kJoinTokens / kGroup + 1 of them.
